@@ -19,7 +19,7 @@ LIB_PATH = Path(os.environ["FMS_LIBRARY"]) if os.environ.get("FMS_LIBRARY") else
     PKG / "libflashmaxsim_sm100.so"
 HEADER = PKG.parent / "include" / "fms.h"
 
-F32, F16, BF16, F64 = 0, 1, 2, 3
+F32, F16, BF16, F64, I8 = 0, 1, 2, 3, 4
 ATOMIC_UNIFIED, INVGRID = 0, 1
 
 DTYPE_CODE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float64: F64}
@@ -32,6 +32,8 @@ _P = C.c_void_p
 _i = C.c_int
 _i64 = C.c_int64
 _d = C.c_double
+_f = C.c_float
+_u32 = C.c_uint32
 _sz = C.c_size_t
 
 # argtypes of every exported entry point (mirrors include/fms.h)
@@ -76,6 +78,18 @@ SIGNATURES = {
                                            _P, _i, _P, _P, _i64, _P, _sz, _P]),
     "fms_topk_merge": (_i, [_P, _P, _i, _i, _i, _P, _P, _P]),
     "fms_candidates_finalize_neg": (_i, [_P, _i64, _i, _i, _d, _P, _P]),
+    # token encoder
+    "fms_gated_ffn_workspace_size": (_sz, [_i64, _i, _i, _i]),
+    "fms_gated_ffn_fwd": (_i, [_i, _P, _P, _P, _i64, _i, _i, _i, _P, _P, _sz, _P]),
+    "fms_gated_ffn_bwd": (_i, [_i, _P, _P, _P, _P, _i64, _i, _i, _i, _P, _P, _P, _P, _sz, _P]),
+    "fms_norm_residual_fwd": (_i, [_i, _i, _i, _P, _P, _P, _P, _P, _P, _P, _i64, _i64, _i, _f, _f,
+                                   _P, _P, _P, _P]),
+    "fms_norm_residual_bwd_workspace_size": (_sz, [_i64, _i64, _i]),
+    "fms_norm_residual_bwd": (_i, [_i, _i, _i, _P, _P, _P, _P, _P, _P, _i64, _i64, _i, _f, _P, _P,
+                                   _P, _P, _P, _P, _P, _P, _P, _P, _P, _sz, _P]),
+    "fms_int8_linear_workspace_size": (_sz, [_i, _i64, _i, _i]),
+    "fms_int8_linear_fwd": (_i, [_i, _P, _P, _P, _P, _P, _i64, _i, _i, _i, _P, _P, _sz, _P]),
+    "fms_adamw_step": (_i, [_i, _i, _P, _i64, _d, _d, _d, _d, _d, _u32, _P, _P]),
     # multi-GPU (NCCL)
     "fms_nccl_available": (_i, []),
     "fms_last_nccl_error": (C.c_char_p, []),

@@ -1,0 +1,181 @@
+"""AdamW over many tensors in one launch, moments in 32 bits or in 8 (no reference
+counterpart: the reference leaves the training step to the caller).
+
+    adamw_step(params, grads, exp_avgs, exp_avg_sqs, step=t, lr=...)   the step
+    AdamW(params, lr=..., bits=8).step()                               its state kept
+
+An 8-bit moment is a pair (codes, scales): codes float8_e4m3fn in the parameter's
+shape, scales float32 (ceil(n / 256),), value = code * scale over runs of 256
+values; the second moment's codes are those of its square root.
+"""
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+from . import _lib
+from .errors import ArgumentError, DimensionMismatch
+
+BLOCK = 256
+_FLOAT = (torch.float32, torch.float16, torch.bfloat16)
+_RECORD = np.dtype([("p", "u8"), ("g", "u8"), ("copy", "u8"), ("m", "u8"), ("v", "u8"),
+                    ("ms", "u8"), ("vs", "u8"), ("n", "i8"), ("pt", "i4"), ("gt", "i4"),
+                    ("ct", "i4"), ("reserved", "i4")])
+
+
+def _same_device(dev, *lists):
+    i = dev.index
+    for ts in lists:
+        for t in ts:
+            if t.get_device() != i:
+                raise ArgumentError("adamw_step: all tensors must live on one CUDA device")
+            if not t.is_contiguous():
+                raise ArgumentError("adamw_step: tensors are updated in place and must be contiguous")
+
+
+@torch.no_grad()
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.9, 0.999),
+               eps=1e-8, weight_decay=1e-2, seed=0, copies=None, grad_scale=None):
+    """One AdamW step (decoupled weight decay) in place over lists of tensors:
+
+        m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+        p = (1 - lr wd) p - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+
+    params and grads are float32, float16 or bfloat16.  exp_avgs and exp_avg_sqs
+    are lists of float32 tensors, or of (codes, scales) pairs of 8-bit moments
+    (`moments8`), whose codes are rounded stochastically by (seed, step).  copies
+    (16-bit tensors, or None) receive the new parameters in their type.  step
+    counts from 1.  grad_scale, a float32 tensor of one value, multiplies the
+    gradients (a clipping factor, an inverse loss scale)."""
+    params, grads = list(params), list(grads)
+    exp_avgs, exp_avg_sqs = list(exp_avgs), list(exp_avg_sqs)
+    n = len(params)
+    copies = None if copies is None else list(copies)
+    if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n) or \
+            (copies is not None and len(copies) != n):
+        raise DimensionMismatch("adamw_step: lists must have one entry per parameter")
+    b1, b2 = betas
+    if not (0 <= b1 < 1 and 0 <= b2 < 1) or not eps >= 0 or int(step) < 1:
+        raise ArgumentError("adamw_step: betas must be in [0, 1), eps >= 0 and step >= 1")
+    if n == 0:
+        return
+    dev = params[0].device
+    if dev.type != "cuda":
+        raise ArgumentError("adamw_step runs on CUDA tensors only")
+    eight = isinstance(exp_avgs[0], (tuple, list))
+    if eight:
+        if not all(isinstance(s, (tuple, list)) and len(s) == 2 for s in exp_avgs + exp_avg_sqs):
+            raise ArgumentError("adamw_step: moments must all be tensors or all (codes, scales)")
+        ms, vs = [s[1] for s in exp_avgs], [s[1] for s in exp_avg_sqs]
+        m, v = [s[0] for s in exp_avgs], [s[0] for s in exp_avg_sqs]
+        _same_device(dev, ms, vs)
+        if any(s.dtype != torch.float32 for s in ms + vs):
+            raise ArgumentError("adamw_step: scales of 8-bit moments must be float32")
+    else:
+        m, v = exp_avgs, exp_avg_sqs
+        if not all(isinstance(s, torch.Tensor) for s in m + v):
+            raise ArgumentError("adamw_step: moments must all be tensors or all (codes, scales)")
+    _same_device(dev, params, grads, m, v, copies or ())
+    want = torch.float8_e4m3fn if eight else torch.float32
+    if any(s.dtype != want for s in m + v):
+        raise ArgumentError(f"adamw_step: moments must hold {want}")
+    if any(t.dtype not in _FLOAT for t in params + grads):
+        raise ArgumentError("adamw_step: parameters and gradients must be float32, float16 or bfloat16")
+    if copies is not None and any(t.dtype not in (torch.float16, torch.bfloat16) for t in copies):
+        raise ArgumentError("adamw_step: copies must be float16 or bfloat16")
+    table = np.zeros(n, _RECORD)
+    sizes = [t.numel() for t in params]
+    for ts in (grads, m, v, copies):
+        if ts is not None and [t.numel() for t in ts] != sizes:
+            raise DimensionMismatch("adamw_step: gradients, moments and copies must have their parameter's size")
+    code = _lib.DTYPE_CODE
+    table["n"] = sizes
+    for k, ts in (("p", params), ("g", grads), ("copy", copies), ("m", m), ("v", v)):
+        if ts is not None:
+            table[k] = [t.data_ptr() for t in ts]
+    table["pt"] = [code[t.dtype] for t in params]
+    table["gt"] = [code[t.dtype] for t in grads]
+    if copies is not None:
+        table["ct"] = [code[t.dtype] for t in copies]
+    if eight:
+        blocks = [-(-s // BLOCK) for s in sizes]
+        if [s.numel() for s in ms] != blocks or [s.numel() for s in vs] != blocks:
+            raise DimensionMismatch("adamw_step: 8-bit moments need one scale per 256 values")
+        table["ms"], table["vs"] = [s.data_ptr() for s in ms], [s.data_ptr() for s in vs]
+    if grad_scale is not None:
+        if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
+            raise ArgumentError("adamw_step: grad_scale must be a float32 tensor of one value")
+        _same_device(dev, [grad_scale])
+    torch.autograd.graph.increment_version(params + m + v + (copies or []))
+    args = (8 if eight else 32, n, table.ctypes.data, int(step), float(lr), float(b1), float(b2),
+            float(eps), float(weight_decay), int(seed) & 0xFFFFFFFF, _lib.ptr(grad_scale))
+    if torch.cuda.current_device() == dev.index:
+        _lib.call("fms_adamw_step", *args, _lib.stream_of(dev))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call("fms_adamw_step", *args, _lib.stream_of(dev))
+
+
+def moments8(p):
+    """A zero 8-bit moment (codes, scales) of parameter p."""
+    return (torch.zeros(p.shape, dtype=torch.float8_e4m3fn, device=p.device),
+            torch.zeros(-(-p.numel() // BLOCK), dtype=torch.float32, device=p.device))
+
+
+class AdamW:
+    """AdamW over a list of parameters, its moments kept in `bits` (32 or 8) each.
+
+    `step()` reads each parameter's .grad (or the list given); parameters without
+    one are left alone.  With `copies`, 16-bit tensors beside float32 parameters
+    receive the new values (the weights that the model computes with).  Moments
+    are made at a parameter's first step."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=32,
+                 seed=0, copies=None):
+        if bits not in (32, 8):
+            raise ArgumentError(f"AdamW: bits must be 32 or 8, got {bits!r}")
+        self.params = list(params)
+        self.copies = None if copies is None else list(copies)
+        if self.copies is not None and len(self.copies) != len(self.params):
+            raise DimensionMismatch("AdamW: one copy per parameter")
+        self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
+        self.bits, self.seed = bits, seed
+        self.steps = [0] * len(self.params)  # each parameter's own: its bias correction
+        self.exp_avgs = [None] * len(self.params)
+        self.exp_avg_sqs = [None] * len(self.params)
+
+    def _moment(self, p):
+        return moments8(p) if self.bits == 8 else \
+            torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+
+    def step(self, grads=None, grad_scale=None):
+        grads = [p.grad for p in self.params] if grads is None else list(grads)
+        if len(grads) != len(self.params):
+            raise DimensionMismatch("AdamW: one gradient per parameter")
+        at = [k for k, g in enumerate(grads) if g is not None]
+        for k in at:
+            if self.exp_avgs[k] is None:
+                self.exp_avgs[k] = self._moment(self.params[k])
+                self.exp_avg_sqs[k] = self._moment(self.params[k])
+            self.steps[k] += 1
+        for t in sorted({self.steps[k] for k in at}):
+            pick = lambda ts: [ts[k] for k in at if self.steps[k] == t]  # noqa: B023, E731
+            adamw_step([p.detach() for p in pick(self.params)], pick(grads), pick(self.exp_avgs),
+                       pick(self.exp_avg_sqs), step=t, lr=self.lr, betas=self.betas, eps=self.eps,
+                       weight_decay=self.weight_decay, seed=self.seed,
+                       copies=None if self.copies is None else pick(self.copies),
+                       grad_scale=grad_scale)
+
+    def zero_grad(self):
+        for p in self.params:
+            p.grad = None
+
+    def state_dict(self):
+        return {"steps": list(self.steps), "bits": self.bits, "exp_avgs": list(self.exp_avgs),
+                "exp_avg_sqs": list(self.exp_avg_sqs)}
+
+    def load_state_dict(self, state):
+        if state["bits"] != self.bits or len(state["exp_avgs"]) != len(self.params):
+            raise ArgumentError("AdamW: the state is of another width or number of parameters")
+        self.steps = list(state["steps"])
+        self.exp_avgs, self.exp_avg_sqs = list(state["exp_avgs"]), list(state["exp_avg_sqs"])

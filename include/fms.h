@@ -40,7 +40,15 @@ extern "C" {
 
 typedef struct CUstream_st* fms_stream_t; /* identical to cudaStream_t */
 
-enum fms_dtype { FMS_F32 = 0, FMS_F16 = 1, FMS_BF16 = 2, FMS_F64 = 3 };
+/* FMS_I8 is taken by fms_int8_linear_fwd only. */
+enum fms_dtype { FMS_F32 = 0, FMS_F16 = 1, FMS_BF16 = 2, FMS_F64 = 3, FMS_I8 = 4 };
+
+/* Activations of the gated feed-forward block: x sigmoid(x); x Phi(x) with the
+   error function; its tanh form; max(x, 0). */
+enum fms_activation { FMS_ACT_SILU = 0, FMS_ACT_GELU = 1, FMS_ACT_GELU_TANH = 2, FMS_ACT_RELU = 3 };
+
+/* Norms: v / sqrt(mean(v^2) + eps), or (v - mean) / sqrt(var + eps). */
+enum fms_norm { FMS_NORM_RMS = 0, FMS_NORM_LAYER = 1 };
 
 /* BackwardStrategy (types.jl:8-17) */
 enum fms_backward { FMS_ATOMIC_UNIFIED = 0, FMS_INVGRID = 1 };
@@ -273,6 +281,93 @@ int fms_topk_merge(const float* vals, const int32_t* ids, int k, int nq, int nsh
    all-reduce(max) of S the slots that are invalid globally get `neg`. */
 int fms_candidates_finalize_neg(const int32_t* idxs, int64_t N, int C, int B, double neg,
                                 float* S, fms_stream_t stream);
+
+/* ------------------------------------------------------------- token encoder
+   No reference counterpart (the reference scores token features that the caller
+   brings): the block that makes the features, its training step and its INT8
+   serving form.  Arrays are row-major with tokens as rows, (rows, dim)
+   contiguous, which is the column-major (dim, rows) of the entry points above. */
+
+/* Gated feed-forward block, FMS_F16 or FMS_BF16:
+     h (rows, hidden) = a(x Wg^T) * (x Wu^T),  x (rows, dim), Wg and Wu (hidden, dim),
+   float32 sums, h rounded once.  The backward pass computes the products again
+   (nothing is kept from the forward pass) and writes dx, dw_gate and dw_up in
+   full; a NULL one is left out.  The gradients of both products are rounded to
+   the inputs' type between the two steps of the backward pass.
+   Workspace: fms_gated_ffn_workspace_size (backward 0 or 1). */
+size_t fms_gated_ffn_workspace_size(int64_t rows, int dim, int hidden, int backward);
+int fms_gated_ffn_fwd(int dtype, const void* x, const void* w_gate, const void* w_up, int64_t rows,
+                      int dim, int hidden, int act, void* h, void* workspace, size_t ws_bytes,
+                      fms_stream_t stream);
+int fms_gated_ffn_bwd(int dtype, const void* x, const void* w_gate, const void* w_up, const void* dh,
+                      int64_t rows, int dim, int hidden, int act, void* dx, void* dw_gate,
+                      void* dw_up, void* workspace, size_t ws_bytes, fms_stream_t stream);
+
+/* The norms around a block with its gate and residual scale:
+     z = scale * x + gate * N(h; w_post, b_post),  y = N(z; w_pre, b_pre)
+   x, h, z, y (rows, dim) in dtype (FMS_F32, FMS_F16 or FMS_BF16); the vectors in
+   vdtype (dtype or FMS_F32).  gate (groups, dim) holds one vector for each run of
+   rows / groups rows (groups divides rows; 1 without a gate), NULL = ones; biases
+   may be NULL.  y is the norm of z before z is rounded.  stats (4, rows) float32,
+   when not NULL, keeps the rows' means and reciprocal deviations for the backward
+   pass.  Gradient outputs of vectors may be NULL; dz and dy may be NULL (zero).
+   Sums over rows are taken in a fixed order.  Workspace of the backward pass:
+   fms_norm_residual_bwd_workspace_size. */
+int fms_norm_residual_fwd(int dtype, int vdtype, int kind, const void* x, const void* h,
+                          const void* w_post, const void* b_post, const void* w_pre,
+                          const void* b_pre, const void* gate, int64_t groups, int64_t rows, int dim,
+                          float eps, float scale, void* z, void* y, float* stats,
+                          fms_stream_t stream);
+size_t fms_norm_residual_bwd_workspace_size(int64_t rows, int64_t groups, int dim);
+int fms_norm_residual_bwd(int dtype, int vdtype, int kind, const void* x, const void* h,
+                          const void* w_post, const void* b_post, const void* w_pre,
+                          const void* gate, int64_t groups, int64_t rows, int dim, float scale,
+                          const float* stats, const void* dz, const void* dy, void* dx, void* dh,
+                          void* dw_post, void* db_post, void* dw_pre, void* db_pre, void* dgate,
+                          void* workspace, size_t ws_bytes, fms_stream_t stream);
+
+/* Linear layer in 8-bit integers, one scale per token and one per output channel:
+     y[t,c] = (sx_t * sw_c) * float(sum_k xc[t,k] * wc[c,k]) + bias_c
+   w_codes (out, dim) with w_scales (out,) float32 -- the codes and scales of
+   fms_quantize_int8 over the weight's rows; y (rows, out) and bias (out,) in
+   y_dtype (FMS_F32, FMS_F16 or FMS_BF16; bias may be NULL).  x is FMS_I8 codes with
+   x_scales, or float features that are quantised per token inside the call, in
+   float32 whatever their type (scale = max(absmax, 1e-8) * (1/127), ties to even); a
+   token with an infinity or a NaN gives NaN.  dim is 1 .. FMS_INT8_LINEAR_MAX_DIM
+   (the int32 sums are exact up to there).  Workspace: fms_int8_linear_workspace_size. */
+#define FMS_INT8_LINEAR_MAX_DIM 131071
+size_t fms_int8_linear_workspace_size(int x_dtype, int64_t rows, int dim, int out);
+int fms_int8_linear_fwd(int x_dtype, const void* x, const float* x_scales, const int8_t* w_codes,
+                        const float* w_scales, const void* bias, int64_t rows, int dim, int out,
+                        int y_dtype, void* y, void* workspace, size_t ws_bytes, fms_stream_t stream);
+
+/* One AdamW step over many tensors (contiguous, n values each), in place:
+     m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
+     p = (1 - lr wd) p - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+   with g = grad * (*grad_scale) when grad_scale (a device float) is not NULL.
+   p and g are FMS_F32, FMS_F16 or FMS_BF16; copy, when not NULL, receives p in a
+   16-bit type as well.  bits 32: m and v are float32.  bits 8: m and v hold e4m3
+   codes of m and of sqrt(v), m_scales and v_scales one float32 per 256 values
+   (value = code * scale); codes are rounded stochastically from (seed, step, the
+   tensor's place in the list, the value's place in the tensor).  `tensors` is a
+   host array that the call reads before it returns. */
+typedef struct fms_adamw_tensor {
+  void* p;
+  const void* g;
+  void* copy;
+  void* m;
+  void* v;
+  float* m_scales;
+  float* v_scales;
+  int64_t n;
+  int32_t p_dtype;
+  int32_t g_dtype;
+  int32_t copy_dtype;
+  int32_t reserved;
+} fms_adamw_tensor;
+int fms_adamw_step(int bits, int ntensors, const fms_adamw_tensor* tensors, int64_t step, double lr,
+                   double beta1, double beta2, double eps, double weight_decay, uint32_t seed,
+                   const float* grad_scale, fms_stream_t stream);
 
 /* ------------------------------------------------------------ multi-GPU (NCCL)
    No reference counterpart (the reference is single-device): galleries sharded
