@@ -106,7 +106,9 @@ int fms_device_error(int reset) {
   const int a = read_device_error(reset);
   const int b = read_i8tc_device_error(reset);
   const int c = read_gal_device_error(reset);
-  return a != 0 ? a : (b != 0 ? b : c);
+  const int d = read_ffn_device_error(reset);
+  const int e = read_lin8_device_error(reset);
+  return a != 0 ? a : b != 0 ? b : c != 0 ? c : d != 0 ? d : e;
 }
 
 int fms_pair_fwd(int dtype, const void* q, const void* d, const uint8_t* qmask,

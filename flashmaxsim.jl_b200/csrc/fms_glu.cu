@@ -5,99 +5,134 @@
 //   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
 //
 // x (rows, dim), Wg and Wu (hidden, dim), h (rows, hidden), 16-bit; sums in
-// float32.  g and u are not kept for the backward pass but computed again: that
-// is one more pair of products, and saves rounding them to 16 bits and
-// 4 * rows * hidden bytes between the passes.
+// float32.  One kernel makes both projections of a tile into one accumulator (its
+// columns are those of Wg and of Wu) and applies the activation and the product as
+// it leaves TMEM.  g and u are not kept for the backward pass but computed again by
+// the same kernel with another epilogue: one more pair of products, against rounding
+// g and u to 16 bits (which would double the gradients' error) and 4 * rows * hidden
+// bytes between the passes.  dg and du are rounded to the inputs' type, the type of
+// the products they enter.
 #include "fms_act.cuh"
+#include "fms_gemm_tc.cuh"
 #include "fms_internal.h"
 
 namespace fms {
 namespace glu {
 
-constexpr int TILE = 64, KT = 16, NT = 256;  // output tile, K step, threads
+using gemm::Tile;
 
-// One 64 x 64 tile of C = sum over the operand pairs of A(m,k) B(k,n), float32
-// sums, 4 x 4 per thread.  A element (m,k) at a[m*sam + k*sak], B (k,n) at
-// b[k*sbk + n*sbn].
-template <typename T>
-struct Strided {
-  const T* a;
-  const T* b;
-  int64_t sam, sak, sbk, sbn;
+// h = a(g) u, or with BWD dg = dh u a'(g) and du = dh a(g).
+template <typename T, int ACT, bool BWD>
+struct HiddenEpi {
+  struct Params {
+    const T* dh;
+    T *o0, *o1;         // h, or dg and du
+    int64_t rows;
+    int hidden, ldo;    // columns; elements between the rows of the outputs
+    int wide, wide_dh;  // rows start on 32 bytes
+  };
+  template <int BN>
+  static __device__ __forceinline__ void run(const Params& p, const Tile& t, int64_t row, int half, uint32_t addr) {
+#pragma unroll 1
+    for (int c = half; c < BN / 64; c += 2) {
+      __syncwarp();
+      uint32_t g[32], u[32];
+      gemm::load32(addr + c * 32, g);
+      gemm::load32(addr + BN / 2 + c * 32, u);
+      const int col = t.n * (BN / 2) + c * 32;
+      const int n = row < p.rows ? p.hidden - col : 0;
+      if (n <= 0) continue;
+      uint32_t o[16], o1[16], d[16];
+      if (BWD) gemm::load_row32(p.dh + row * p.hidden + col, d, n, p.wide_dh);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float a0, a1, b0, b1;
+        const float g0 = __uint_as_float(g[2 * i]), g1 = __uint_as_float(g[2 * i + 1]);
+        const float u0 = __uint_as_float(u[2 * i]), u1 = __uint_as_float(u[2 * i + 1]);
+        act_eval<ACT, BWD>(g0, a0, b0);
+        act_eval<ACT, BWD>(g1, a1, b1);
+        if (BWD) {
+          const float2 e = gemm::unpack2<T>(d[i]);
+          o[i] = gemm::pack2<T>(e.x * u0 * b0, e.y * u1 * b1);
+          o1[i] = gemm::pack2<T>(e.x * a0, e.y * a1);
+        } else {
+          o[i] = gemm::pack2<T>(a0 * u0, a1 * u1);
+        }
+      }
+      gemm::store_row32(p.o0 + row * p.ldo + col, o, n, p.wide);
+      if (BWD) gemm::store_row32(p.o1 + row * p.ldo + col, o1, n, p.wide);
+    }
+  }
 };
 
+// The accumulator as it is, in T, or in float32 where the sum is split (`part` then
+// holds one (rows, cols) matrix after the other).  STACK: the rows are those of two
+// outputs, `pad` rows of tiles each.
+template <typename T, bool STACK>
+struct StoreEpi {
+  struct Params {
+    T *o0, *o1;
+    float* part;
+    int64_t rows, pad;
+    int cols;
+    int wide;
+  };
+  template <int BN>
+  static __device__ __forceinline__ void run(const Params& p, const Tile& t, int64_t row, int half, uint32_t addr) {
+    T* out = p.o0;
+    int64_t at = t.split * (STACK ? 2 : 1) * p.rows;
+    if (STACK && row >= p.pad) {
+      row -= p.pad;
+      out = p.o1;
+      at += p.rows;
+    }
+#pragma unroll 1
+    for (int c = half; c < BN / 32; c += 2) {
+      __syncwarp();
+      uint32_t v[32];
+      gemm::load32(addr + c * 32, v);
+      const int col = t.n * BN + c * 32;
+      const int n = row < p.rows ? p.cols - col : 0;
+      if (n <= 0) continue;
+      if (p.part) {
+        float* q = p.part + (at + row) * p.cols + col;
+        if (n >= 32 && p.wide) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            reinterpret_cast<uint4*>(q)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (i < n) q[i] = __uint_as_float(v[i]);
+        }
+      } else if (out) {
+        uint32_t o[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = gemm::pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+        gemm::store_row32(out + row * p.cols + col, o, n, p.wide);
+      }
+    }
+  }
+};
+
+// Sum of the parts of a split product, in order.
 template <typename T>
-__device__ __forceinline__ void tile_product(const Strided<T>& s, int64_t m0, int64_t n0, int64_t M, int64_t N,
-                                             int64_t K, float (*As)[TILE + 4], float (*Bs)[TILE + 4],
-                                             float (&acc)[4][4]) {
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  for (int64_t k0 = 0; k0 < K; k0 += KT) {
-    for (int e = threadIdx.x; e < TILE * KT; e += NT) {
-      // neighbouring threads along the operand's contiguous axis
-      const int mi = s.sak == 1 ? e / KT : e % TILE, ka = s.sak == 1 ? e % KT : e / TILE;
-      const int ni = s.sbk == 1 ? e / KT : e % TILE, kb = s.sbk == 1 ? e % KT : e / TILE;
-      As[ka][mi] = m0 + mi < M && k0 + ka < K ? Tr<T>::to(s.a[(m0 + mi) * s.sam + (k0 + ka) * s.sak]) : 0.f;
-      Bs[kb][ni] = n0 + ni < N && k0 + kb < K ? Tr<T>::to(s.b[(k0 + kb) * s.sbk + (n0 + ni) * s.sbn]) : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < KT; ++k) {
-      float a[4], b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = As[k][ty * 4 + i], b[i] = Bs[k][tx * 4 + i];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-    }
-    __syncthreads();
+__global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int64_t each, T* o0, T* o1) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < 2 * each; i += (int64_t)gridDim.x * 256) {
+    T* o = i < each ? o0 : o1;
+    if (!o) continue;
+    float s = 0.f;
+    for (int k = 0; k < splits; ++k) s += part[k * 2 * each + i];
+    o[i < each ? i : i - each] = Tr<T>::from(s);
   }
 }
 
-// Both projections and the activation; with dh the gradients of g and u instead of h.
-template <typename T, int ACT, bool BWD>
-__global__ void __launch_bounds__(NT) hidden_kernel(const T* x, const T* wg, const T* wu, const T* dh, int64_t rows,
-                                                    int dim, int hidden, T* h, T* dg, T* du) {
-  __shared__ float As[KT][TILE + 4], Bs[KT][TILE + 4];
-  const int64_t m0 = (int64_t)blockIdx.x * TILE, n0 = (int64_t)blockIdx.y * TILE;
-  float g[4][4] = {}, u[4][4] = {};
-  tile_product<T>({x, wg, dim, 1, 1, dim}, m0, n0, rows, hidden, dim, As, Bs, g);
-  tile_product<T>({x, wu, dim, 1, 1, dim}, m0, n0, rows, hidden, dim, As, Bs, u);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      if (m >= rows || n >= hidden) continue;
-      float a, da = 0.f;
-      act_eval<ACT, BWD>(g[i][j], a, da);
-      if (BWD) {
-        const float d = Tr<T>::to(dh[m * hidden + n]);
-        dg[m * hidden + n] = Tr<T>::from(d * u[i][j] * da);
-        du[m * hidden + n] = Tr<T>::from(d * a);
-      } else {
-        h[m * hidden + n] = Tr<T>::from(a * u[i][j]);
-      }
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(NT) product_kernel(Strided<T> s1, Strided<T> s2, int pairs, int64_t M, int64_t N,
-                                                     int64_t K, T* c) {
-  __shared__ float As[KT][TILE + 4], Bs[KT][TILE + 4];
-  const int64_t m0 = (int64_t)blockIdx.x * TILE, n0 = (int64_t)blockIdx.y * TILE;
-  float acc[4][4] = {};
-  tile_product<T>(s1, m0, n0, M, N, K, As, Bs, acc);
-  if (pairs == 2) tile_product<T>(s2, m0, n0, M, N, K, As, Bs, acc);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      if (m < M && n < N) c[m * N + n] = Tr<T>::from(acc[i][j]);
-    }
+// Rows of `dim` elements copied to rows `ld` apart, for operands whose rows do not
+// start on 16 bytes as TMA asks.
+__global__ void __launch_bounds__(256) pitch_kernel(const uint16_t* src, int64_t rows, int dim, uint16_t* dst, int ld) {
+  const int64_t n = rows * dim;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    dst[i / dim * ld + i % dim] = src[i];
 }
 
 struct Args {
@@ -105,58 +140,205 @@ struct Args {
   int64_t rows;
   int dim, hidden;
   void *h, *dx, *dwg, *dwu;
-  void* ws;
+  char* ws;
 };
 
-static dim3 grid(int64_t M, int64_t N) { return dim3((unsigned)((M + TILE - 1) / TILE), (unsigned)((N + TILE - 1) / TILE)); }
+static int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+static int64_t tiles(int64_t n, int64_t t) { return (n + t - 1) / t; }
 
-template <typename T, int ACT>
-static cudaError_t run(const Args& p, bool bwd, cudaStream_t s) {
-  const T *x = (const T*)p.x, *wg = (const T*)p.wg, *wu = (const T*)p.wu;
-  T* dg = (T*)p.ws;
-  T* du = dg + p.rows * p.hidden;
-  const int64_t R = p.rows;
-  const int D = p.dim, F = p.hidden;
-  if (R > 0 && F > 0) {
-    if (bwd)
-      hidden_kernel<T, ACT, true><<<grid(R, F), NT, 0, s>>>(x, wg, wu, (const T*)p.dh, R, D, F, nullptr, dg, du);
-    else
-      hidden_kernel<T, ACT, false><<<grid(R, F), NT, 0, s>>>(x, wg, wu, nullptr, R, D, F, (T*)p.h, nullptr, nullptr);
+// Parts of the sum over rows for the weights' gradients: enough to give every pair of
+// SMs a tile of about the same length, at least 16 blocks of 64 rows each.
+static int weight_splits(int64_t rows, int dim, int hidden) {
+  const int64_t t = 2 * tiles(hidden, 256) * tiles(dim, 256), pairs = device_sm_count() / 2, kb = tiles(rows, 64);
+  int64_t best = 1;
+  double cost = 1e30;
+  for (int64_t s = 1; s <= 16 && (s == 1 || kb / s >= 16); ++s) {
+    const double c = (double)tiles(t * s, pairs) * ((double)kb / s + 8.0);  // + a tile's start and end
+    if (c < cost * 0.97) cost = c, best = s;
   }
-  if (bwd && D > 0) {
-    if (p.dx && R > 0)
-      product_kernel<T><<<grid(R, D), NT, 0, s>>>({dg, wg, F, 1, D, 1}, {du, wu, F, 1, D, 1}, 2, R, D, F, (T*)p.dx);
-    if (p.dwg && F > 0)
-      product_kernel<T><<<grid(F, D), NT, 0, s>>>({dg, x, 1, F, D, 1}, {}, 1, F, D, R, (T*)p.dwg);
-    if (p.dwu && F > 0)
-      product_kernel<T><<<grid(F, D), NT, 0, s>>>({du, x, 1, F, D, 1}, {}, 1, F, D, R, (T*)p.dwu);
+  return (int)best;
+}
+
+struct Space {
+  size_t x, wg, wu, dg, du, part, total;
+  int ldd, ldh, splits;
+};
+// Offsets of the workspace.  The padded copies have their place whenever the width
+// asks for them or a pointer might (the size is known without the pointers).
+static Space space(int64_t rows, int dim, int hidden, bool bwd) {
+  Space s{};
+  s.ldd = (int)up(dim, 8);
+  s.ldh = (int)up(hidden, 8);
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t o = at;
+    at += (size_t)up((int64_t)n, 256);
+    return o;
+  };
+  s.x = take((size_t)rows * s.ldd * 2);
+  s.wg = take((size_t)hidden * s.ldd * 2);
+  s.wu = take((size_t)hidden * s.ldd * 2);
+  if (bwd) {
+    s.dg = take((size_t)rows * s.ldh * 2);
+    s.du = take((size_t)rows * s.ldh * 2);
+    s.splits = weight_splits(rows, dim, hidden);
+    if (s.splits > 1) s.part = take((size_t)s.splits * 2 * hidden * dim * 4);
   }
+  s.total = at;
+  return s;
+}
+
+static bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// The operand with rows that TMA can read: as it is, or copied.
+static const void* pitched(const void* p, int64_t rows, int dim, int ld, char* copy, cudaStream_t s) {
+  if (dim == ld && aligned(p, 16)) return p;
+  int64_t b = tiles(rows * dim, 256 * 8);
+  if (b > 148 * 16) b = 148 * 16;
+  pitch_kernel<<<(unsigned)b, 256, 0, s>>>((const uint16_t*)p, rows, dim, (uint16_t*)copy, ld);
+  return copy;
+}
+
+template <typename T, int ACT, bool BWD, int CG, int BN>
+static cudaError_t hidden_pass(int dtype, const void* x, const void* wg, const void* wu, int ldd, const Args& p, T* o0,
+                               T* o1, int ldo, cudaStream_t s) {
+  CUtensorMap a, b0, b1;
+  const int box = BN / 2;
+  if (!gemm::make_map(&a, dtype, x, p.dim, p.rows, (int64_t)ldd * 2, 128) ||
+      !gemm::make_map(&b0, dtype, wg, p.dim, p.hidden, (int64_t)ldd * 2, box) ||
+      !gemm::make_map(&b1, dtype, wu, p.dim, p.hidden, (int64_t)ldd * 2, box))
+    return cudaErrorNotSupported;
+  gemm::Work w{};
+  w.mt = (int)tiles(p.rows, 128 * CG);
+  w.nt = (int)tiles(p.hidden, BN / 2);
+  w.splits = 1;
+  w.kb = (int)tiles(p.dim, 64);
+  w.idesc = gemm::idesc_f16(dtype, 128 * CG, BN, false, false);
+  typename HiddenEpi<T, ACT, BWD>::Params e{};
+  e.dh = (const T*)p.dh;
+  e.o0 = o0;
+  e.o1 = o1;
+  e.rows = p.rows;
+  e.hidden = p.hidden;
+  e.ldo = ldo;
+  e.wide = ldo % 16 == 0 && aligned(o0, 32) && (!BWD || aligned(o1, 32));
+  e.wide_dh = p.hidden % 16 == 0 && aligned(p.dh, 32);
+  return gemm::launch<gemm::OP_PAIR_B, CG, BN, false, false, false, HiddenEpi<T, ACT, BWD>>(a, a, b0, b1, w, e,
+                                                                                            device_sm_count(), s);
+}
+
+template <typename T, int ACT, bool BWD>
+static cudaError_t hidden_any(int dtype, const void* x, const void* wg, const void* wu, int ldd, const Args& p, T* o0,
+                              T* o1, int ldo, cudaStream_t s) {
+  return hidden_pass<T, ACT, BWD, 2, 256>(dtype, x, wg, wu, ldd, p, o0, o1, ldo, s);
+}
+
+// dx = dg Wg + du Wu: the weights as they lie are the second operand with its rows
+// along the sum.
+template <typename T>
+static cudaError_t input_gradient(int dtype, const T* dg, const T* du, const void* wg, const void* wu, int ldd, int ldh,
+                                  const Args& p, cudaStream_t s) {
+  CUtensorMap a0, a1, b0, b1;
+  if (!gemm::make_map(&a0, dtype, dg, p.hidden, p.rows, (int64_t)ldh * 2, 128) ||
+      !gemm::make_map(&a1, dtype, du, p.hidden, p.rows, (int64_t)ldh * 2, 128) ||
+      !gemm::make_map(&b0, dtype, wg, p.dim, p.hidden, (int64_t)ldd * 2, 64) ||
+      !gemm::make_map(&b1, dtype, wu, p.dim, p.hidden, (int64_t)ldd * 2, 64))
+    return cudaErrorNotSupported;
+  gemm::Work w{};
+  w.mt = (int)tiles(p.rows, 256);
+  w.nt = (int)tiles(p.dim, 256);
+  w.splits = 1;
+  w.kb0 = (int)tiles(p.hidden, 64);
+  w.kb = 2 * w.kb0;
+  w.idesc = gemm::idesc_f16(dtype, 256, 256, false, true);
+  typename StoreEpi<T, false>::Params e{};
+  e.o0 = (T*)p.dx;
+  e.rows = p.rows;
+  e.cols = p.dim;
+  e.wide = p.dim % 16 == 0 && aligned(p.dx, 32);
+  return gemm::launch<gemm::OP_SUM, 2, 256, false, true, false, StoreEpi<T, false>>(a0, a1, b0, b1, w, e,
+                                                                                    device_sm_count(), s);
+}
+
+// dWg = dg^T x over dWu = du^T x: both operands have their rows along the sum.
+template <typename T>
+static cudaError_t weight_gradients(int dtype, const T* dg, const T* du, const void* x, int ldd, int ldh, int splits,
+                                    float* part, const Args& p, cudaStream_t s) {
+  CUtensorMap a0, a1, b;
+  if (!gemm::make_map(&a0, dtype, dg, p.hidden, p.rows, (int64_t)ldh * 2, 64) ||
+      !gemm::make_map(&a1, dtype, du, p.hidden, p.rows, (int64_t)ldh * 2, 64) ||
+      !gemm::make_map(&b, dtype, x, p.dim, p.rows, (int64_t)ldd * 2, 64))
+    return cudaErrorNotSupported;
+  gemm::Work w{};
+  w.mt0 = (int)tiles(p.hidden, 256);
+  w.mt = 2 * w.mt0;
+  w.nt = (int)tiles(p.dim, 256);
+  w.splits = splits;
+  w.kb = (int)tiles(p.rows, 64);
+  w.idesc = gemm::idesc_f16(dtype, 256, 256, true, true);
+  typename StoreEpi<T, true>::Params e{};
+  e.o0 = (T*)p.dwg;
+  e.o1 = (T*)p.dwu;
+  e.part = splits > 1 ? part : nullptr;
+  e.rows = p.hidden;
+  e.pad = (int64_t)w.mt0 * 256;
+  e.cols = p.dim;
+  e.wide = e.part ? p.dim % 4 == 0 : p.dim % 16 == 0 && aligned(p.dwg, 32) && aligned(p.dwu, 32);
+  const cudaError_t err = gemm::launch<gemm::OP_STACK_A, 2, 256, true, true, false, StoreEpi<T, true>>(
+      a0, a1, b, b, w, e, device_sm_count(), s);
+  if (err != cudaSuccess || splits == 1) return err;
+  const int64_t each = (int64_t)p.hidden * p.dim;
+  int64_t blocks = tiles(2 * each, 256 * 4);
+  if (blocks > device_sm_count() * 8) blocks = device_sm_count() * 8;
+  join_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(part, splits, each, (T*)p.dwg, (T*)p.dwu);
   return cudaGetLastError();
 }
 
+template <typename T, int ACT>
+static cudaError_t run(int dtype, const Args& p, bool bwd, cudaStream_t s) {
+  const Space L = space(p.rows, p.dim, p.hidden, bwd);
+  const void* x = pitched(p.x, p.rows, p.dim, L.ldd, p.ws + L.x, s);
+  const void* wg = pitched(p.wg, p.hidden, p.dim, L.ldd, p.ws + L.wg, s);
+  const void* wu = pitched(p.wu, p.hidden, p.dim, L.ldd, p.ws + L.wu, s);
+  if (!bwd) return hidden_any<T, ACT, false>(dtype, x, wg, wu, L.ldd, p, (T*)p.h, nullptr, p.hidden, s);
+  T *dg = (T*)(p.ws + L.dg), *du = (T*)(p.ws + L.du);
+  cudaError_t e = hidden_any<T, ACT, true>(dtype, x, wg, wu, L.ldd, p, dg, du, L.ldh, s);
+  if (e == cudaSuccess && p.dx) e = input_gradient<T>(dtype, dg, du, wg, wu, L.ldd, L.ldh, p, s);
+  if (e == cudaSuccess && (p.dwg || p.dwu))
+    e = weight_gradients<T>(dtype, dg, du, x, L.ldd, L.ldh, L.splits, (float*)(p.ws + L.part), p, s);
+  return e;
+}
+
 template <typename T>
-static cudaError_t run_act(int act, const Args& p, bool bwd, cudaStream_t s) {
+static cudaError_t run_act(int dtype, int act, const Args& p, bool bwd, cudaStream_t s) {
   switch (act) {
-    case FMS_ACT_SILU: return run<T, FMS_ACT_SILU>(p, bwd, s);
-    case FMS_ACT_GELU: return run<T, FMS_ACT_GELU>(p, bwd, s);
-    case FMS_ACT_GELU_TANH: return run<T, FMS_ACT_GELU_TANH>(p, bwd, s);
-    default: return run<T, FMS_ACT_RELU>(p, bwd, s);
+    case FMS_ACT_SILU: return run<T, FMS_ACT_SILU>(dtype, p, bwd, s);
+    case FMS_ACT_GELU: return run<T, FMS_ACT_GELU>(dtype, p, bwd, s);
+    case FMS_ACT_GELU_TANH: return run<T, FMS_ACT_GELU_TANH>(dtype, p, bwd, s);
+    default: return run<T, FMS_ACT_RELU>(dtype, p, bwd, s);
   }
 }
 
 static int check(int dtype, int act, int64_t rows, int dim, int hidden) {
   if (dtype != FMS_F16 && dtype != FMS_BF16) return FMS_ERR_DTYPE;
   if (act < FMS_ACT_SILU || act > FMS_ACT_RELU) return FMS_ERR_INVALID;
-  if (rows < 0 || rows > INT32_MAX || dim < 0 || hidden < 0) return FMS_ERR_INVALID;
+  // row and column coordinates of a tile are 32-bit
+  if (rows < 0 || rows > INT32_MAX - 512 || dim < 0 || dim > INT32_MAX - 512 || hidden < 0 || hidden > INT32_MAX - 512)
+    return FMS_ERR_INVALID;
   return FMS_OK;
 }
 
 static int launch(int dtype, int act, const Args& p, bool bwd, cudaStream_t s) {
-  const cudaError_t e = dtype == FMS_F16 ? run_act<__half>(act, p, bwd, s) : run_act<__nv_bfloat16>(act, p, bwd, s);
-  return e == cudaSuccess ? FMS_OK : (int)e;
+  if (device_cc() != 100) return FMS_ERR_UNSUPPORTED;
+  const cudaError_t e =
+      dtype == FMS_F16 ? run_act<__half>(dtype, act, p, bwd, s) : run_act<__nv_bfloat16>(dtype, act, p, bwd, s);
+  return e == cudaSuccess ? FMS_OK : e == cudaErrorNotSupported ? FMS_ERR_UNSUPPORTED : (int)e;
 }
 
 }  // namespace glu
+
+int read_ffn_device_error(int reset) { return gemm::read_error(reset); }
+
 }  // namespace fms
 
 using namespace fms;
@@ -164,8 +346,8 @@ using namespace fms;
 extern "C" {
 
 size_t fms_gated_ffn_workspace_size(int64_t rows, int dim, int hidden, int backward) {
-  if (rows <= 0 || dim < 0 || hidden <= 0) return 0;
-  return backward ? (size_t)rows * hidden * 2 * 2 : 0;
+  if (rows <= 0 || dim <= 0 || hidden <= 0) return 0;
+  return glu::space(rows, dim, hidden, backward != 0).total;
 }
 
 int fms_gated_ffn_fwd(int dtype, const void* x, const void* w_gate, const void* w_up, int64_t rows, int dim,
@@ -174,9 +356,14 @@ int fms_gated_ffn_fwd(int dtype, const void* x, const void* w_gate, const void* 
   if (st != FMS_OK) return st;
   if (rows == 0 || hidden == 0) return FMS_OK;
   if (!h || (dim > 0 && (!x || !w_gate || !w_up))) return FMS_ERR_INVALID;
-  if (ws_bytes < fms_gated_ffn_workspace_size(rows, dim, hidden, 0)) return FMS_ERR_WORKSPACE;
-  return glu::launch(dtype, act, {x, w_gate, w_up, nullptr, rows, dim, hidden, h, nullptr, nullptr, nullptr, workspace},
-                     false, (cudaStream_t)stream);
+  if (dim == 0) {  // empty sums
+    const cudaError_t e = cudaMemsetAsync(h, 0, (size_t)rows * hidden * 2, (cudaStream_t)stream);
+    return e == cudaSuccess ? FMS_OK : (int)e;
+  }
+  if (!workspace || ws_bytes < fms_gated_ffn_workspace_size(rows, dim, hidden, 0)) return FMS_ERR_WORKSPACE;
+  return glu::launch(dtype, act,
+                     {x, w_gate, w_up, nullptr, rows, dim, hidden, h, nullptr, nullptr, nullptr, (char*)workspace}, false,
+                     (cudaStream_t)stream);
 }
 
 int fms_gated_ffn_bwd(int dtype, const void* x, const void* w_gate, const void* w_up, const void* dh, int64_t rows,
@@ -185,10 +372,16 @@ int fms_gated_ffn_bwd(int dtype, const void* x, const void* w_gate, const void* 
   const int st = glu::check(dtype, act, rows, dim, hidden);
   if (st != FMS_OK) return st;
   if (dim == 0) return FMS_OK;
-  if (rows > 0 && hidden > 0 && (!x || !w_gate || !w_up || !dh)) return FMS_ERR_INVALID;
-  const size_t need = fms_gated_ffn_workspace_size(rows, dim, hidden, 1);
-  if (need && (!workspace || ws_bytes < need)) return FMS_ERR_WORKSPACE;
-  return glu::launch(dtype, act, {x, w_gate, w_up, dh, rows, dim, hidden, nullptr, dx, dw_gate, dw_up, workspace},
+  if (rows == 0 || hidden == 0) {  // empty sums
+    cudaError_t e = cudaSuccess;
+    if (dx) e = cudaMemsetAsync(dx, 0, (size_t)rows * dim * 2, (cudaStream_t)stream);
+    if (dw_gate && e == cudaSuccess) e = cudaMemsetAsync(dw_gate, 0, (size_t)hidden * dim * 2, (cudaStream_t)stream);
+    if (dw_up && e == cudaSuccess) e = cudaMemsetAsync(dw_up, 0, (size_t)hidden * dim * 2, (cudaStream_t)stream);
+    return e == cudaSuccess ? FMS_OK : (int)e;
+  }
+  if (!x || !w_gate || !w_up || !dh) return FMS_ERR_INVALID;
+  if (!workspace || ws_bytes < fms_gated_ffn_workspace_size(rows, dim, hidden, 1)) return FMS_ERR_WORKSPACE;
+  return glu::launch(dtype, act, {x, w_gate, w_up, dh, rows, dim, hidden, nullptr, dx, dw_gate, dw_up, (char*)workspace},
                      true, (cudaStream_t)stream);
 }
 

@@ -35,6 +35,15 @@ bool scan_gallery_supported(int dtype, const ScanParams& p);
 cudaError_t launch_scan_gallery(int dtype, const ScanParams& p, cudaStream_t s);
 int read_gal_device_error(int reset);
 
+// The token encoder's matrix-product engine (fms_gemm_tc.cuh).
+namespace gemm {
+// 2-D TMA map over (inner, outer) elements, `pitch` bytes between the outer rows (a
+// multiple of 16), boxes of 128 bytes x `box` rows, 128-byte swizzle, zeros outside.
+bool make_map(CUtensorMap* m, int dtype, const void* base, int64_t inner, int64_t outer, int64_t pitch, int box);
+}  // namespace gemm
+int read_ffn_device_error(int reset);
+int read_lin8_device_error(int reset);
+
 cudaError_t launch_inv_counts(int dtype, const uint8_t* qmask, int Tq, int B, void* inv_n,
                               cudaStream_t s);
 

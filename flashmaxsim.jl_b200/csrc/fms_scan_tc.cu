@@ -965,6 +965,24 @@ bool make_tmap_i8(CUtensorMap* m, const void* base, int dim, int64_t rows, int b
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+namespace gemm {
+bool make_map(CUtensorMap* m, int dtype, const void* base, int64_t inner, int64_t outer, int64_t pitch, int box) {
+  tc::EncodeTiledFn enc = tc::encode_fn();
+  if (!enc) return false;
+  const bool i8 = dtype == FMS_I8;
+  cuuint64_t gdim[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+  cuuint64_t gstride[1] = {(cuuint64_t)pitch};
+  cuuint32_t tile[2] = {i8 ? 128u : 64u, (cuuint32_t)box};
+  cuuint32_t estride[2] = {1, 1};
+  const CUtensorMapDataType t = i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : dtype == FMS_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return enc(m, t, 2, const_cast<void*>(base), gdim, gstride, tile, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+}  // namespace gemm
+
 int read_device_error(int reset) {
   int v = 0;
   cudaError_t e = cudaMemcpyFromSymbol(&v, g_tc_error, sizeof(int));
