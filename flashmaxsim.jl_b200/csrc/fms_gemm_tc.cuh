@@ -460,6 +460,29 @@ inline uint32_t idesc_f16(int dtype, int M, int N, bool a_mn, bool b_mn) {
          ((uint32_t)(M >> 4) << 24);
 }
 
+// Which tile a product takes.  Measured per block of the sum: the 256 x 256 tile of a CTA
+// pair takes the MMAs' 512 cycles, narrower tiles what their loads take at about 60
+// bytes per cycle and SM; a launch adds about 2500 cycles for its first loads and last
+// epilogue.  Pairs of 256 columns win where there are tiles for all SMs; few rows or
+// columns take narrower tiles that use more SMs.
+struct Shape {
+  int cg, bn;
+  double step;
+};
+constexpr Shape SHAPES[] = {{2, 256, 546.0}, {2, 128, 410.0}, {1, 64, 410.0}};
+inline int pick_shape(int64_t rows, int64_t cols, int kb, int sms) {
+  int best = 0;
+  double cost = 1e300;
+  for (int i = 0; i < 3; ++i) {
+    const Shape& h = SHAPES[i];
+    const int64_t t = ((rows + 128 * h.cg - 1) / (128 * h.cg)) * ((cols + h.bn - 1) / h.bn);
+    const int64_t slots = sms / h.cg;
+    const double c = (double)((t + slots - 1) / slots) * (kb * h.step + 600.0) + 2500.0;
+    if (c < cost) cost = c, best = i;
+  }
+  return best;
+}
+
 template <int OP, int CG, int BN, bool A_MN, bool B_MN, bool I8, class Epi>
 cudaError_t launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& b0, const CUtensorMap& b1,
                    const Work& w, const typename Epi::Params& e, int sms, cudaStream_t s) {

@@ -6,93 +6,392 @@
 // The integer sum is exact (int32; the entry point bounds K).  Float inputs are
 // quantised per token first, in float32 whatever their type: scale =
 // max(absmax, 1e-8) * (1/127), code = round to nearest even of x / scale.
-#include "fms_common.cuh"
+//
+// Up to FEW tokens one kernel quantises and multiplies on the CUDA cores (bound by
+// reading the weights once); more go through a quantising pass and the tcgen05
+// engine (kind::i8, scales in the epilogue).
+#include "fms_gemm_tc.cuh"
 #include "fms_internal.h"
 
 namespace fms {
 namespace lin8 {
 
-// One warp per token: absmax, then codes.
+constexpr int FEW = 8;  // tokens of the CUDA-core kernel
+
+// ------------------------------------------------------------------ quantising
+
+// 127 / absmax and its inverse for one token.  A token that holds an infinity or a
+// NaN has no scale: all its outputs are NaN.
+struct Scale {
+  float s, inv;
+};
+__device__ __forceinline__ Scale make_scale(uint32_t top_bits) {
+  const float am = __uint_as_float(top_bits);
+  Scale r;
+  r.s = am <= 3.402823466e38f ? fmaxf(am, 1e-8f) * (1.f / 127.f) : NAN;
+  r.inv = __frcp_rn(r.s);
+  return r;
+}
+// The code of x in the low byte.  x / s as a product with the reciprocal and one
+// correction by the remainder (Markstein's division step), which is the correctly
+// rounded quotient; adding 1.5 * 2^23 rounds it to a whole number, ties to even.
+// |x / s| <= 127 (1 + 2^-23), so no clamp is needed.
+__device__ __forceinline__ uint32_t code(float x, Scale s) {
+  const float q = x * s.inv;
+  const float r = fmaf(-q, s.s, x);
+  return __float_as_uint(fmaf(r, s.inv, q) + 12582912.f);
+}
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// The values of one 16-byte vector as float32: 8 of a 16-bit type, 4 of float32.
 template <typename T>
-__global__ void __launch_bounds__(256) quantize_kernel(const T* x, int64_t rows, int K, int8_t* codes, float* scales) {
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  static __device__ __forceinline__ void get(uint4 v, float (&f)[N]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (N == 4) {
+        f[i] = __uint_as_float(w[i]);
+      } else {
+        const float2 p = gemm::unpack2<T>(w[i]);
+        f[2 * i] = p.x;
+        f[2 * i + 1] = p.y;
+      }
+    }
+  }
+};
+
+// One warp per token with the row in registers: NV 16-byte vectors per lane.  Bound by
+// memory: the row is read once and its codes written once.
+template <typename T, int NV>
+__global__ void __launch_bounds__(256) quantize_kernel(const T* x, int64_t rows, int K, int8_t* codes, int pitch,
+                                                       float* scales) {
+  constexpr int N = Vec<T>::N;
   const int lane = threadIdx.x & 31;
   const int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (t >= rows) return;
-  const T* xt = x + t * K;
+  const uint4* xt = reinterpret_cast<const uint4*>(x + t * K);
+  uint4 v[NV];
   uint32_t top = 0;  // bits of the largest |x|; as whole numbers a NaN's are above infinity's
-  for (int k = lane; k < K; k += 32) top = max(top, __float_as_uint(fabsf(Tr<T>::to(xt[k]))));
-  top = __reduce_max_sync(0xffffffffu, top);
-  const float am = __uint_as_float(top);
-  // a token that holds an infinity or a NaN has no scale: all its outputs are NaN
-  const float sc = am <= 3.402823466e38f ? fmaxf(am, 1e-8f) * (1.f / 127.f) : NAN;
-  for (int k = lane; k < K; k += 32) {
-    const float v = rintf(fminf(fmaxf(Tr<T>::to(xt[k]) / sc, -127.f), 127.f));
-    codes[t * K + k] = (int8_t)v;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    v[i] = make_uint4(0, 0, 0, 0);
+    if ((i * 32 + lane) * N < K) v[i] = __ldg(xt + i * 32 + lane);
   }
-  if (lane == 0) scales[t] = sc;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float f[N];
+    Vec<T>::get(v[i], f);
+#pragma unroll
+    for (int j = 0; j < N; ++j) top = max(top, abs_bits(f[j]));
+  }
+  const Scale s = make_scale(__reduce_max_sync(0xffffffffu, top));
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int k = (i * 32 + lane) * N;
+    if (k >= K) continue;
+    float f[N];
+    Vec<T>::get(v[i], f);
+    uint32_t c[N / 4];
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j)
+      c[j] = pack4(code(f[4 * j], s), code(f[4 * j + 1], s), code(f[4 * j + 2], s), code(f[4 * j + 3], s));
+    if constexpr (N == 8) *reinterpret_cast<uint2*>(codes + t * pitch + k) = make_uint2(c[0], c[1]);
+    else *reinterpret_cast<uint32_t*>(codes + t * pitch + k) = c[0];
+  }
+  if (lane == 0) scales[t] = s.s;
 }
 
-constexpr int TILE = 64, KT = 32, NT = 256;
-
+// Rows of any width and start, one block each, read twice.
 template <typename T>
-__global__ void __launch_bounds__(NT) linear_kernel(const int8_t* xc, const float* sx, const int8_t* wc,
-                                                    const float* sw, const T* bias, int64_t rows, int K, int C, T* y) {
-  __shared__ int32_t Xs[KT / 4][TILE + 1], Ws[KT / 4][TILE + 1];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int64_t m0 = (int64_t)blockIdx.x * TILE;
-  const int n0 = blockIdx.y * TILE;
-  int32_t acc[4][4] = {};
-  for (int k0 = 0; k0 < K; k0 += KT) {
-    for (int e = threadIdx.x; e < TILE * (KT / 4); e += NT) {
-      const int kk = e % (KT / 4), i = e / (KT / 4);
-      uint32_t xw = 0, ww = 0;
-      for (int b = 0; b < 4; ++b) {
-        const int k = k0 + kk * 4 + b;
-        if (k < K && m0 + i < rows) xw |= (uint32_t)(uint8_t)xc[(m0 + i) * K + k] << (8 * b);
-        if (k < K && n0 + i < C) ww |= (uint32_t)(uint8_t)wc[(int64_t)(n0 + i) * K + k] << (8 * b);
-      }
-      Xs[kk][i] = (int32_t)xw;
-      Ws[kk][i] = (int32_t)ww;
-    }
+__global__ void __launch_bounds__(256) quantize_any_kernel(const T* x, int64_t rows, int K, int8_t* codes, int pitch,
+                                                           float* scales) {
+  __shared__ uint32_t part[8];
+  for (int64_t t = blockIdx.x; t < rows; t += gridDim.x) {
+    const T* xt = x + t * K;
+    uint32_t top = 0;
+    for (int k = threadIdx.x; k < K; k += 256) top = max(top, abs_bits(Tr<T>::to(xt[k])));
+    top = __reduce_max_sync(0xffffffffu, top);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < KT / 4; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(Xs[k][ty + 16 * i], Ws[k][tx + 16 * j], acc[i][j]);
-    __syncthreads();
+    for (int i = 0; i < 8; ++i) top = max(top, part[i]);
+    const Scale s = make_scale(top);
+    for (int k = threadIdx.x; k < K; k += 256) codes[t * pitch + k] = (int8_t)code(Tr<T>::to(xt[k]), s);
+    if (threadIdx.x == 0) scales[t] = s.s;
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t t = m0 + ty + 16 * i;
-      const int c = n0 + tx + 16 * j;
-      if (t >= rows || c >= C) continue;
-      float v = (sx[t] * sw[c]) * (float)acc[i][j];
-      if (bias) v += Tr<T>::to(bias[c]);
-      y[t * C + c] = Tr<T>::from(v);
-    }
 }
+
+// ------------------------------------------------------------------ a few tokens
+
+// Every block quantises all tokens for itself (they are a few KB) into shared memory;
+// then one warp per output channel: 16-byte pieces of the weight's row against the same
+// pieces of every token, dp4a, and a sum over the lanes.  VEC: bytes of a piece that the
+// weights' alignment allows.
+template <typename X, typename Y, int NTOK, int VEC>
+__global__ void __launch_bounds__(256) few_kernel(const X* x, const float* x_scales, const int8_t* wc, const float* sw,
+                                                  const Y* bias, int rows, int K, int C, Y* y) {
+  extern __shared__ __align__(16) unsigned char codes_s[];  // (rows, pitch)
+  __shared__ float sx[NTOK];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pitch = (K + 15) & ~15;
+  for (int t = warp; t < rows; t += 8) {
+    unsigned char* ct = codes_s + t * pitch;
+    if constexpr (sizeof(X) == 1) {
+      for (int k = lane; k < pitch; k += 32) ct[k] = k < K ? (unsigned char)x[(int64_t)t * K + k] : 0;
+      if (lane == 0) sx[t] = x_scales[t];
+    } else {
+      const X* xt = x + (int64_t)t * K;
+      uint32_t top = 0;
+      for (int k = lane; k < K; k += 32) top = max(top, abs_bits(Tr<X>::to(xt[k])));
+      const Scale s = make_scale(__reduce_max_sync(0xffffffffu, top));
+      for (int k = lane; k < pitch; k += 32) ct[k] = k < K ? (unsigned char)code(Tr<X>::to(xt[k]), s) : 0;
+      if (lane == 0) sx[t] = s.s;
+    }
+  }
+  __syncthreads();
+  for (int c = blockIdx.x * 8 + warp; c < C; c += gridDim.x * 8) {
+    const int8_t* w = wc + (int64_t)c * K;
+    int32_t acc[NTOK];
+#pragma unroll
+    for (int t = 0; t < NTOK; ++t) acc[t] = 0;
+#pragma unroll 2
+    for (int k = lane * VEC; k < K; k += 32 * VEC) {
+      if constexpr (VEC == 16) {
+        const int4 v = __ldg(reinterpret_cast<const int4*>(w + k));
+#pragma unroll
+        for (int t = 0; t < NTOK; ++t) {
+          if (t >= rows) break;
+          const int4 q = *reinterpret_cast<const int4*>(codes_s + t * pitch + k);
+          acc[t] = __dp4a(v.x, q.x, __dp4a(v.y, q.y, __dp4a(v.z, q.z, __dp4a(v.w, q.w, acc[t]))));
+        }
+      } else if constexpr (VEC == 4) {
+        const int v = __ldg(reinterpret_cast<const int*>(w + k));
+#pragma unroll
+        for (int t = 0; t < NTOK; ++t) {
+          if (t >= rows) break;
+          acc[t] = __dp4a(v, *reinterpret_cast<const int*>(codes_s + t * pitch + k), acc[t]);
+        }
+      } else {
+        const int v = w[k];
+#pragma unroll
+        for (int t = 0; t < NTOK; ++t) {
+          if (t >= rows) break;
+          acc[t] += v * (int)(int8_t)codes_s[t * pitch + k];
+        }
+      }
+    }
+    int32_t mine = 0;
+#pragma unroll
+    for (int t = 0; t < NTOK; ++t) {
+      if (t >= rows) break;
+      const int32_t sum = __reduce_add_sync(0xffffffffu, acc[t]);
+      if (lane == t) mine = sum;
+    }
+    if (lane < rows) {
+      float v = (sx[lane] * sw[c]) * (float)mine;
+      if (bias) v += Tr<Y>::to(bias[c]);
+      y[(int64_t)lane * C + c] = Tr<Y>::from(v);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ the engine's epilogue
+
+template <typename Y>
+struct ScaleEpi {
+  struct Params {
+    const float *sx, *sw;
+    const Y* bias;
+    Y* y;
+    int64_t rows;
+    int cols;
+    int wide;       // rows of y start on 32 bytes
+  };
+  template <int BN>
+  static __device__ __forceinline__ void run(const Params& p, const gemm::Tile& t, int64_t row, int half,
+                                             uint32_t addr) {
+    const float sx = row < p.rows ? __ldg(p.sx + row) : 0.f;
+#pragma unroll 1
+    for (int c = half; c < BN / 32; c += 2) {
+      __syncwarp();
+      uint32_t v[32];
+      gemm::load32(addr + c * 32, v);
+      const int col = t.n * BN + c * 32;
+      const int n = row < p.rows ? p.cols - col : 0;
+      if (n <= 0) continue;
+      float f[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const int at = i < n ? col + i : col;
+        f[i] = (sx * __ldg(p.sw + at)) * (float)(int32_t)v[i];
+        if (p.bias) f[i] += Tr<Y>::to(p.bias[at]);
+      }
+      Y* out = p.y + row * p.cols + col;
+      if constexpr (sizeof(Y) == 2) {
+        uint32_t o[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = gemm::pack2<Y>(f[2 * i], f[2 * i + 1]);
+        gemm::store_row32(out, o, n, p.wide);
+      } else {
+        uint32_t o[16];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // 16 floats are 32 half-words
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(f[16 * h + i]);
+          gemm::store_row32(reinterpret_cast<uint16_t*>(out + 16 * h), o, 2 * (n - 16 * h), p.wide);
+        }
+      }
+    }
+  }
+};
+
+// ------------------------------------------------------------------ host side
 
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+static int pitch_of(int K) { return (K + 15) & ~15; }
+static bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-template <typename T>
-static void quantize(const void* x, int64_t rows, int K, int8_t* codes, float* scales, cudaStream_t s) {
-  quantize_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, s>>>((const T*)x, rows, K, codes, scales);
+// Bytes copied to rows `pitch` apart, for codes whose rows do not start on 16 bytes.
+__global__ void __launch_bounds__(256) pitch_kernel(const int8_t* src, int64_t rows, int K, int8_t* dst, int pitch) {
+  const int64_t n = rows * K;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    dst[i / K * pitch + i % K] = src[i];
+}
+static const int8_t* pitched(const int8_t* p, int64_t rows, int K, int8_t* copy, cudaStream_t s) {
+  if (K % 16 == 0 && aligned(p, 16)) return p;
+  int64_t b = (rows * K + 2047) / 2048;
+  if (b > 148 * 16) b = 148 * 16;
+  pitch_kernel<<<(unsigned)b, 256, 0, s>>>(p, rows, K, copy, pitch_of(K));
+  return copy;
 }
 
 template <typename T>
-static void linear(const int8_t* xc, const float* sx, const int8_t* wc, const float* sw, const void* bias, int64_t rows,
-                   int K, int C, void* y, cudaStream_t s) {
-  const dim3 grid((unsigned)((rows + TILE - 1) / TILE), (unsigned)((C + TILE - 1) / TILE));
-  linear_kernel<T><<<grid, NT, 0, s>>>(xc, sx, wc, sw, (const T*)bias, rows, K, C, (T*)y);
+static void quantize(const void* xv, int64_t rows, int K, int8_t* codes, float* scales, cudaStream_t s) {
+  const T* x = (const T*)xv;
+  constexpr int N = Vec<T>::N;
+  const unsigned blocks = (unsigned)((rows + 7) / 8);
+  const int pitch = pitch_of(K);
+  if (K % N != 0 || !aligned(x, 16) || K > 32 * N * 16) {
+    quantize_any_kernel<T><<<(unsigned)(rows < 148 * 8 ? rows : 148 * 8), 256, 0, s>>>(x, rows, K, codes, pitch, scales);
+    return;
+  }
+  const int nv = (K + 32 * N - 1) / (32 * N);
+  if (nv <= 1) quantize_kernel<T, 1><<<blocks, 256, 0, s>>>(x, rows, K, codes, pitch, scales);
+  else if (nv <= 2) quantize_kernel<T, 2><<<blocks, 256, 0, s>>>(x, rows, K, codes, pitch, scales);
+  else if (nv <= 4) quantize_kernel<T, 4><<<blocks, 256, 0, s>>>(x, rows, K, codes, pitch, scales);
+  else if (nv <= 8) quantize_kernel<T, 8><<<blocks, 256, 0, s>>>(x, rows, K, codes, pitch, scales);
+  else quantize_kernel<T, 16><<<blocks, 256, 0, s>>>(x, rows, K, codes, pitch, scales);
+}
+
+struct Args {
+  const void* x;
+  const float* x_scales;
+  const int8_t* wc;
+  const float* sw;
+  const void* bias;
+  int64_t rows;
+  int K, C;
+  void* y;
+  char* ws;
+};
+
+struct Space {
+  size_t codes, scales, w, total;
+};
+static bool few(int64_t rows, int K) { return rows <= FEW && rows * pitch_of(K) <= 40 * 1024; }
+static Space space(int x_dtype, int64_t rows, int K, int C) {
+  Space s{};
+  if (few(rows, K)) return s;
+  s.scales = align256((size_t)rows * pitch_of(K));
+  s.w = s.scales + (x_dtype == FMS_I8 ? 0 : align256((size_t)rows * 4));
+  s.total = s.w + align256((size_t)C * pitch_of(K));
+  return s;
+}
+
+template <typename X, typename Y, int NTOK>
+static cudaError_t run_few(const Args& p, cudaStream_t s) {
+  int blocks = (p.C + 7) / 8;
+  const int most = device_sm_count() * 4;
+  if (blocks > most) blocks = most;
+  const int smem = (int)p.rows * pitch_of(p.K);
+  const X* x = (const X*)p.x;
+  const Y* bias = (const Y*)p.bias;
+  Y* y = (Y*)p.y;
+  if (p.K % 16 == 0 && aligned(p.wc, 16))
+    few_kernel<X, Y, NTOK, 16><<<blocks, 256, smem, s>>>(x, p.x_scales, p.wc, p.sw, bias, (int)p.rows, p.K, p.C, y);
+  else if (p.K % 4 == 0 && aligned(p.wc, 4))
+    few_kernel<X, Y, NTOK, 4><<<blocks, 256, smem, s>>>(x, p.x_scales, p.wc, p.sw, bias, (int)p.rows, p.K, p.C, y);
+  else
+    few_kernel<X, Y, NTOK, 1><<<blocks, 256, smem, s>>>(x, p.x_scales, p.wc, p.sw, bias, (int)p.rows, p.K, p.C, y);
+  return cudaGetLastError();
+}
+
+template <typename Y, int CG, int BN>
+static cudaError_t product(const int8_t* xc, const float* sx, const int8_t* wc, const Args& p, cudaStream_t s) {
+  CUtensorMap a, b;
+  if (!gemm::make_map(&a, FMS_I8, xc, p.K, p.rows, pitch_of(p.K), 128) ||
+      !gemm::make_map(&b, FMS_I8, wc, p.K, p.C, pitch_of(p.K), BN / CG))
+    return cudaErrorNotSupported;
+  gemm::Work w{};
+  w.mt = (int)((p.rows + 128 * CG - 1) / (128 * CG));
+  w.nt = (p.C + BN - 1) / BN;
+  w.splits = 1;
+  w.kb = (p.K + 127) / 128;
+  w.idesc = ptx::idesc_i8(128 * CG, BN);
+  typename ScaleEpi<Y>::Params e{};
+  e.sx = sx;
+  e.sw = p.sw;
+  e.bias = (const Y*)p.bias;
+  e.y = (Y*)p.y;
+  e.rows = p.rows;
+  e.cols = p.C;
+  e.wide = (p.C * sizeof(Y)) % 32 == 0 && aligned(p.y, 32);
+  return gemm::launch<gemm::OP_ONE, CG, BN, false, false, true, ScaleEpi<Y>>(a, a, b, b, w, e, device_sm_count(), s);
+}
+
+template <typename X, typename Y>
+static cudaError_t run(const Args& p, cudaStream_t s) {
+  if (few(p.rows, p.K)) return p.rows == 1 ? run_few<X, Y, 1>(p, s) : run_few<X, Y, FEW>(p, s);
+  const Space L = space(sizeof(X) == 1 ? FMS_I8 : FMS_F32, p.rows, p.K, p.C);
+  int8_t* codes = (int8_t*)(p.ws + L.codes);
+  const int8_t* xc;
+  const float* sx;
+  if constexpr (sizeof(X) == 1) {
+    xc = pitched((const int8_t*)p.x, p.rows, p.K, codes, s);
+    sx = p.x_scales;
+  } else {
+    float* sc = (float*)(p.ws + L.scales);
+    quantize<X>(p.x, p.rows, p.K, codes, sc, s);
+    xc = codes;
+    sx = sc;
+  }
+  const int8_t* wc = pitched(p.wc, p.C, p.K, (int8_t*)(p.ws + L.w), s);
+  switch (gemm::pick_shape(p.rows, p.C, (p.K + 127) / 128, device_sm_count())) {
+    case 0: return product<Y, 2, 256>(xc, sx, wc, p, s);
+    case 1: return product<Y, 2, 128>(xc, sx, wc, p, s);
+    default: return product<Y, 1, 64>(xc, sx, wc, p, s);
+  }
+}
+
+template <typename Y>
+static cudaError_t run_x(int x_dtype, const Args& p, cudaStream_t s) {
+  switch (x_dtype) {
+    case FMS_I8: return run<int8_t, Y>(p, s);
+    case FMS_F32: return run<float, Y>(p, s);
+    case FMS_F16: return run<__half, Y>(p, s);
+    default: return run<__nv_bfloat16, Y>(p, s);
+  }
 }
 
 }  // namespace lin8
 
-int read_lin8_device_error(int) { return 0; }
+int read_lin8_device_error(int reset) { return gemm::read_error(reset); }
 
 }  // namespace fms
 
@@ -101,8 +400,8 @@ using namespace fms;
 extern "C" {
 
 size_t fms_int8_linear_workspace_size(int x_dtype, int64_t rows, int dim, int out) {
-  if (rows <= 0 || dim <= 0 || out <= 0 || x_dtype == FMS_I8) return 0;
-  return lin8::align256((size_t)rows * dim) + (size_t)rows * 4;
+  if (rows <= 0 || dim <= 0 || out <= 0) return 0;
+  return lin8::space(x_dtype, rows, dim, out).total;
 }
 
 int fms_int8_linear_fwd(int x_dtype, const void* x, const float* x_scales, const int8_t* w_codes, const float* w_scales,
@@ -110,29 +409,19 @@ int fms_int8_linear_fwd(int x_dtype, const void* x, const float* x_scales, const
                         size_t ws_bytes, fms_stream_t stream) {
   if (x_dtype != FMS_I8 && x_dtype != FMS_F32 && x_dtype != FMS_F16 && x_dtype != FMS_BF16) return FMS_ERR_DTYPE;
   if (y_dtype != FMS_F32 && y_dtype != FMS_F16 && y_dtype != FMS_BF16) return FMS_ERR_DTYPE;
-  if (rows < 0 || rows > INT32_MAX || dim < 1 || out < 0) return FMS_ERR_INVALID;
+  if (rows < 0 || rows > INT32_MAX - 512 || dim < 1 || out < 0 || out > INT32_MAX - 512) return FMS_ERR_INVALID;
   if (dim > FMS_INT8_LINEAR_MAX_DIM) return FMS_ERR_TOO_LARGE;
   if (rows == 0 || out == 0) return FMS_OK;
   if (!y || !w_scales || !x || !w_codes || (x_dtype == FMS_I8 && !x_scales)) return FMS_ERR_INVALID;
   const size_t need = fms_int8_linear_workspace_size(x_dtype, rows, dim, out);
   if (need && (!workspace || ws_bytes < need)) return FMS_ERR_WORKSPACE;
+  if (device_cc() != 100) return FMS_ERR_UNSUPPORTED;
+  const lin8::Args p{x, x_scales, w_codes, w_scales, bias, rows, dim, out, y, (char*)workspace};
   cudaStream_t s = (cudaStream_t)stream;
-  const int8_t* xc = (const int8_t*)x;
-  const float* sx = x_scales;
-  if (x_dtype != FMS_I8) {
-    int8_t* c = (int8_t*)workspace;
-    float* sc = (float*)((char*)workspace + lin8::align256((size_t)rows * dim));
-    if (x_dtype == FMS_F32) lin8::quantize<float>(x, rows, dim, c, sc, s);
-    else if (x_dtype == FMS_F16) lin8::quantize<__half>(x, rows, dim, c, sc, s);
-    else lin8::quantize<__nv_bfloat16>(x, rows, dim, c, sc, s);
-    xc = c;
-    sx = sc;
-  }
-  if (y_dtype == FMS_F32) lin8::linear<float>(xc, sx, w_codes, w_scales, bias, rows, dim, out, y, s);
-  else if (y_dtype == FMS_F16) lin8::linear<__half>(xc, sx, w_codes, w_scales, bias, rows, dim, out, y, s);
-  else lin8::linear<__nv_bfloat16>(xc, sx, w_codes, w_scales, bias, rows, dim, out, y, s);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? FMS_OK : (int)e;
+  const cudaError_t e = y_dtype == FMS_F32   ? lin8::run_x<float>(x_dtype, p, s)
+                        : y_dtype == FMS_F16 ? lin8::run_x<__half>(x_dtype, p, s)
+                                             : lin8::run_x<__nv_bfloat16>(x_dtype, p, s);
+  return e == cudaSuccess ? FMS_OK : e == cudaErrorNotSupported ? FMS_ERR_UNSUPPORTED : (int)e;
 }
 
 }  // extern "C"

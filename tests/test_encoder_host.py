@@ -27,7 +27,7 @@ def test_entry_points_reject_before_launching(fms):
     assert L.fms_int8_linear_fwd(3, one, None, one, one, None, 1, 8, 8, 0, one, None, 0, None) == -2
     assert L.fms_int8_linear_fwd(4, one, None, one, one, None, 1, 8, 8, 0, one, None, 0, None) == -1
     assert L.fms_int8_linear_fwd(0, one, None, one, one, None, 1, 0, 8, 0, one, None, 0, None) == -1
-    assert L.fms_int8_linear_fwd(0, one, None, one, one, None, 1, 8, 8, 0, one, None, 0, None) == -4
+    assert L.fms_int8_linear_fwd(0, one, None, one, one, None, 99, 8, 8, 0, one, None, 0, None) == -4
     # adamw: width, step, betas, a tensor without a pointer, none at all
     assert L.fms_adamw_step(16, 0, None, 1, 1e-3, 0.9, 0.99, 1e-8, 0.0, 0, None, None) == -2
     assert L.fms_adamw_step(32, 0, None, 0, 1e-3, 0.9, 0.99, 1e-8, 0.0, 0, None, None) == -1
