@@ -17,94 +17,196 @@
 // T1 = sum dy zhat, T0 = sum dy, from which every vector's gradient follows:
 //   dw_post = sum_g gate S1, db_post = sum_g gate S0, dw_pre = sum T1,
 //   db_pre = sum T0, dgate = w_post S1 + b_post S0.
-// A group's rows are cut into units; each unit writes its sums, and a second
-// kernel adds the units in order, so that results repeat bit for bit.
+// A group's rows are cut into units, one block each; a unit writes its sums, and a
+// second kernel adds the units in order, so that results repeat bit for bit.
+//
+// All of it is bound by memory: a row is read once into registers (forward x and h,
+// backward x, h, dz and dy) and written once; nothing else but the statistics and the
+// units' sums goes out.
 #include "fms_common.cuh"
 #include "fms_internal.h"
 
 namespace fms {
 namespace norm {
 
-constexpr int NT = 256;
-
 struct Params {
   const void *x, *h, *dz, *dy;        // rows in T; dz, dy may be NULL (zero)
-  const void *w_post, *b_post, *w_pre, *b_pre, *gate;  // vectors in V; biases and gate may be NULL
+  const void *w_post, *b_post, *w_pre, *b_pre, *gate;  // vectors in vdt; biases and gate may be NULL
   void *z, *y, *dx, *dh;              // rows in T
-  void *dw_post, *db_post, *dw_pre, *db_pre, *dgate;   // vectors in V, or NULL
+  void *dw_post, *db_post, *dw_pre, *db_pre, *dgate;   // vectors in vdt, or NULL
   float* stats;                       // (4, rows): mean and rstd of h, mean and rstd of z
-  float* part;                        // (4, units, dim)
+  float* part;                        // (4, units, dim): S1, T1, S0, T0
   int64_t rows, per, groups;          // rows per gate vector, gate vectors
   int64_t units;                      // units of the backward pass
   int segs;                           // units per group (0 without rows)
-  int dim;
+  int dim, vdt, layer;
   float eps, scale;
 };
 
-template <typename V>
-__device__ __forceinline__ float vec(const void* p, int64_t i, float none) {
-  return p ? Tr<V>::to(static_cast<const V*>(p)[i]) : none;
-}
-
-// Sum over the block of one or two values, the same on every thread.
-__device__ __forceinline__ float2 block_sum2(float2 v) {
-  __shared__ float2 part[NT / 32];
+// VEC neighbouring values as float32: one 16-byte access, or one value (rows that do not
+// start on 16 bytes).
+template <typename T, int VEC>
+__device__ __forceinline__ void load(const T* p, float (&f)[VEC]) {
+  if constexpr (VEC == 1) {
+    f[0] = Tr<T>::to(*p);
+  } else {
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        f[j] = __uint_as_float(w[j]);
+      } else {
+        const T* t = reinterpret_cast<const T*>(&w[j]);
+        f[2 * j] = Tr<T>::to(t[0]);
+        f[2 * j + 1] = Tr<T>::to(t[1]);
+      }
+    }
   }
-  __syncthreads();  // the last call's reads are done
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float2 t = part[0];
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store(T* p, const float (&f)[VEC]) {
+  if constexpr (VEC == 1) {
+    *p = Tr<T>::from(f[0]);
+  } else {
+    uint32_t w[4];
 #pragma unroll
-  for (int i = 1; i < NT / 32; ++i) t.x += part[i].x, t.y += part[i].y;
-  return t;
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        w[j] = __float_as_uint(f[j]);
+      } else {
+        T t[2] = {Tr<T>::from(f[2 * j]), Tr<T>::from(f[2 * j + 1])};
+        w[j] = *reinterpret_cast<const uint32_t*>(t);
+      }
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+// The same of a weight, bias or gate (in T or float32); `none` where there is none.
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const void* p, int vdt, int64_t at, float none, float (&f)[VEC]) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[j] = none;
+  } else if (vdt == FMS_F32) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[j] = __ldg(static_cast<const float*>(p) + at + j);
+  } else {
+    load<T, VEC>(static_cast<const T*>(p) + at, f);
+  }
+}
+__device__ __forceinline__ float vec1(const void* p, int vdt, int64_t i, float none) {
+  if (p == nullptr) return none;
+  return vdt == FMS_F32   ? static_cast<const float*>(p)[i]
+         : vdt == FMS_F16 ? __half2float(static_cast<const __half*>(p)[i])
+                          : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void put1(void* p, int vdt, int64_t i, float v) {
+  if (p == nullptr) return;
+  if (vdt == FMS_F32) static_cast<float*>(p)[i] = v;
+  else if (vdt == FMS_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// One row per block.
-template <typename T, typename V, bool LAYER>
-__global__ void __launch_bounds__(NT) forward_kernel(Params p) {
-  const int64_t r = blockIdx.x;
+constexpr int MAX_WARPS = 32;
+
+// Sums of two values over the threads of a row, the same on each of them: a warp, or
+// the whole block (one barrier: the partial sums alternate between two places).
+template <bool WARP>
+struct RowSum {
+  float2 (*part)[MAX_WARPS];
+  int turn = 0;
+  __device__ __forceinline__ float2 operator()(float2 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    if (WARP) return v;
+    if ((threadIdx.x & 31) == 0) part[turn][threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int n = blockDim.x >> 5;
+    float2 t = part[turn][0];
+    for (int i = 1; i < n; ++i) t.x += part[turn][i].x, t.y += part[turn][i].y;
+    turn ^= 1;
+    return t;
+  }
+};
+
+// One row per warp (WARP) or block; a thread holds NV runs of VEC values.  A warp takes
+// rows of up to 4 runs per lane (no barriers between the row's sums), a block the wider
+// ones.
+template <typename T, int VEC, int NV, bool WARP>
+__global__ void __launch_bounds__(WARP ? 128 : 1024) forward_kernel(Params p) {
+  __shared__ float2 part[2][MAX_WARPS];
+  RowSum<WARP> sum{part};
+  const int64_t r = WARP ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  if (WARP && r >= p.rows) return;
+  const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, tpr = WARP ? 32 : blockDim.x;
   const int D = p.dim;
+  const float inv_d = 1.f / D;
   const T* x = static_cast<const T*>(p.x) + r * D;
   const T* h = static_cast<const T*>(p.h) + r * D;
-  T* z = static_cast<T*>(p.z) + r * D;
-  T* y = static_cast<T*>(p.y) + r * D;
   const int64_t g0 = (r / p.per) * D;
-  float mh = 0.f, mz = 0.f, s = 0.f;
-  if (LAYER) {
-    for (int c = threadIdx.x; c < D; c += NT) s += Tr<T>::to(h[c]);
-    mh = block_sum2({s, 0.f}).x / D;
+  float z[NV][VEC], v[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * tpr + tid) * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) z[i][j] = v[i][j] = 0.f;
+    if (c < D) {
+      load<T, VEC>(h + c, v[i]);
+      load<T, VEC>(x + c, z[i]);
+    }
   }
-  s = 0.f;
-  for (int c = threadIdx.x; c < D; c += NT) {
-    const float v = Tr<T>::to(h[c]) - mh;
-    s += v * v;
-  }
-  const float rh = rsqrtf(block_sum2({s, 0.f}).x / D + p.eps);
-  auto zval = [&](int c) {
-    const float n = (Tr<T>::to(h[c]) - mh) * rh * vec<V>(p.w_post, c, 1.f) + vec<V>(p.b_post, c, 0.f);
-    return p.scale * Tr<T>::to(x[c]) + vec<V>(p.gate, g0 + c, 1.f) * n;
+  // mean, and the reciprocal deviation of the centred values (two passes over registers)
+  auto stats = [&](float (&a)[NV][VEC], float& mean, float& rstd) {
+    mean = 0.f;
+    if (p.layer) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s += a[i][j];
+      mean = sum({s, 0.f}).x * inv_d;
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float d = (i * tpr + tid) * VEC < D ? a[i][j] - mean : 0.f;
+        s += d * d;
+      }
+    rstd = rsqrtf(sum({s, 0.f}).x * inv_d + p.eps);
   };
-  if (LAYER) {
-    s = 0.f;
-    for (int c = threadIdx.x; c < D; c += NT) s += zval(c);
-    mz = block_sum2({s, 0.f}).x / D;
+  float mh, rh, mz, rz;
+  stats(v, mh, rh);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * tpr + tid) * VEC;
+    if (c >= D) continue;
+    float w[VEC], b[VEC], g[VEC];
+    load_vec<T, VEC>(p.w_post, p.vdt, c, 1.f, w);
+    load_vec<T, VEC>(p.b_post, p.vdt, c, 0.f, b);
+    load_vec<T, VEC>(p.gate, p.vdt, g0 + c, 1.f, g);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) z[i][j] = p.scale * z[i][j] + g[j] * ((v[i][j] - mh) * rh * w[j] + b[j]);
+    store<T, VEC>(static_cast<T*>(p.z) + r * D + c, z[i]);
   }
-  s = 0.f;
-  for (int c = threadIdx.x; c < D; c += NT) {
-    const float v = zval(c) - mz;
-    s += v * v;
+  stats(z, mz, rz);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * tpr + tid) * VEC;
+    if (c >= D) continue;
+    float w[VEC], b[VEC];
+    load_vec<T, VEC>(p.w_pre, p.vdt, c, 1.f, w);
+    load_vec<T, VEC>(p.b_pre, p.vdt, c, 0.f, b);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) z[i][j] = (z[i][j] - mz) * rz * w[j] + b[j];
+    store<T, VEC>(static_cast<T*>(p.y) + r * D + c, z[i]);
   }
-  const float rz = rsqrtf(block_sum2({s, 0.f}).x / D + p.eps);
-  for (int c = threadIdx.x; c < D; c += NT) {
-    const float v = zval(c);
-    z[c] = Tr<T>::from(v);
-    y[c] = Tr<T>::from((v - mz) * rz * vec<V>(p.w_pre, c, 1.f) + vec<V>(p.b_pre, c, 0.f));
-  }
-  if (p.stats && threadIdx.x == 0) {
+  if (p.stats && tid == 0) {
     p.stats[r] = mh;
     p.stats[p.rows + r] = rh;
     p.stats[2 * p.rows + r] = mz;
@@ -112,122 +214,251 @@ __global__ void __launch_bounds__(NT) forward_kernel(Params p) {
   }
 }
 
-// One unit (a run of one group's rows) per block; every thread owns the columns
-// threadIdx.x + i NT of the unit's sums.
-template <typename T, typename V, bool LAYER>
-__global__ void __launch_bounds__(NT) backward_kernel(Params p) {
+// One unit (a run of one group's rows) per block, a row at a time; a thread owns the
+// same NV runs of VEC columns in every row and keeps their sums in registers.  BIAS:
+// S0 and T0 are wanted too.
+template <typename T, int VEC, int NV, bool BIAS>
+__global__ void __launch_bounds__(512) backward_kernel(Params p) {
+  __shared__ float2 part[2][MAX_WARPS];
+  RowSum<false> sum{part};
   const int D = p.dim;
+  const float inv_d = 1.f / D;
   const int64_t group = blockIdx.x / p.segs, seg = blockIdx.x % p.segs;
   const int64_t r0 = group * p.per + p.per * seg / p.segs, r1 = group * p.per + p.per * (seg + 1) / p.segs;
-  float* S1 = p.part + (int64_t)blockIdx.x * D;
-  float* S0 = S1 + p.units * D;
-  float* T1 = S0 + p.units * D;
-  float* T0 = T1 + p.units * D;
-  for (int c = threadIdx.x; c < D; c += NT) S1[c] = S0[c] = T1[c] = T0[c] = 0.f;
-  const int64_t g0 = group * D;
+  float gw[NV][VEC], gb[NV][VEC], wp[NV][VEC];  // gate w_post, gate b_post, w_pre
+  float S1[NV][VEC], T1[NV][VEC], S0[NV][VEC], T0[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * blockDim.x + threadIdx.x) * VEC;
+    float g[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      S1[i][j] = T1[i][j] = S0[i][j] = T0[i][j] = 0.f;
+      gw[i][j] = gb[i][j] = wp[i][j] = g[j] = 0.f;
+    }
+    if (c >= D) continue;
+    load_vec<T, VEC>(p.gate, p.vdt, group * D + c, 1.f, g);
+    load_vec<T, VEC>(p.w_post, p.vdt, c, 1.f, gw[i]);
+    if (BIAS) load_vec<T, VEC>(p.b_post, p.vdt, c, 0.f, gb[i]);
+    load_vec<T, VEC>(p.w_pre, p.vdt, c, 1.f, wp[i]);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) gw[i][j] *= g[j], gb[i][j] *= g[j];
+  }
   for (int64_t r = r0; r < r1; ++r) {
-    const T* x = static_cast<const T*>(p.x) + r * D;
-    const T* h = static_cast<const T*>(p.h) + r * D;
     const float mh = p.stats[r], rh = p.stats[p.rows + r], mz = p.stats[2 * p.rows + r], rz = p.stats[3 * p.rows + r];
-    auto hhat = [&](int c) { return (Tr<T>::to(h[c]) - mh) * rh; };
-    auto gate = [&](int c) { return vec<V>(p.gate, g0 + c, 1.f); };
-    auto zhat = [&](int c) {
-      const float n = hhat(c) * vec<V>(p.w_post, c, 1.f) + vec<V>(p.b_post, c, 0.f);
-      return (p.scale * Tr<T>::to(x[c]) + gate(c) * n - mz) * rz;
-    };
-    auto dyv = [&](int c) { return vec<T>(p.dy, r * D + c, 0.f); };
+    float hh[NV][VEC], zh[NV][VEC], dy[NV][VEC], d[NV][VEC];
     float2 a = {0.f, 0.f};
-    for (int c = threadIdx.x; c < D; c += NT) {
-      const float v = dyv(c) * vec<V>(p.w_pre, c, 1.f);
-      a.x += v * zhat(c);
-      if (LAYER) a.y += v;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * blockDim.x + threadIdx.x) * VEC;
+      const int64_t at = r * D + c;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) hh[i][j] = zh[i][j] = dy[i][j] = d[i][j] = 0.f;
+      if (c >= D) continue;
+      load<T, VEC>(static_cast<const T*>(p.x) + at, zh[i]);
+      load<T, VEC>(static_cast<const T*>(p.h) + at, hh[i]);
+      if (p.dy) load<T, VEC>(static_cast<const T*>(p.dy) + at, dy[i]);
+      if (p.dz) load<T, VEC>(static_cast<const T*>(p.dz) + at, d[i]);
     }
-    a = block_sum2(a);
-    a.x /= D, a.y /= D;
-    auto dzt = [&](int c) {
-      return vec<T>(p.dz, r * D + c, 0.f) + rz * (dyv(c) * vec<V>(p.w_pre, c, 1.f) - a.y - zhat(c) * a.x);
-    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if ((i * (int)blockDim.x + (int)threadIdx.x) * VEC >= D) continue;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        hh[i][j] = (hh[i][j] - mh) * rh;
+        zh[i][j] = (p.scale * zh[i][j] + (hh[i][j] * gw[i][j] + gb[i][j]) - mz) * rz;
+        const float t = dy[i][j] * wp[i][j];
+        a.x += t * zh[i][j];
+        a.y += t;
+      }
+    }
+    a = sum(a);
+    a.x *= inv_d;
+    a.y = p.layer ? a.y * inv_d : 0.f;
     float2 b = {0.f, 0.f};
-    for (int c = threadIdx.x; c < D; c += NT) {
-      const float v = dzt(c) * gate(c) * vec<V>(p.w_post, c, 1.f);
-      b.x += v * hhat(c);
-      if (LAYER) b.y += v;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        d[i][j] += rz * (dy[i][j] * wp[i][j] - a.y - zh[i][j] * a.x);
+        const float e = d[i][j] * gw[i][j];  // 0 past the row's end
+        b.x += e * hh[i][j];
+        b.y += e;
+      }
+    b = sum(b);
+    b.x *= inv_d;
+    b.y = p.layer ? b.y * inv_d : 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * blockDim.x + threadIdx.x) * VEC;
+      if (c >= D) continue;
+      const int64_t at = r * D + c;
+      float o[VEC], q[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        o[j] = p.scale * d[i][j];
+        q[j] = rh * (d[i][j] * gw[i][j] - b.y - hh[i][j] * b.x);
+        S1[i][j] += d[i][j] * hh[i][j];
+        T1[i][j] += dy[i][j] * zh[i][j];
+        if (BIAS) S0[i][j] += d[i][j], T0[i][j] += dy[i][j];
+      }
+      store<T, VEC>(static_cast<T*>(p.dx) + at, o);
+      store<T, VEC>(static_cast<T*>(p.dh) + at, q);
     }
-    b = block_sum2(b);
-    b.x /= D, b.y /= D;
-    for (int c = threadIdx.x; c < D; c += NT) {
-      const float d = dzt(c), hh = hhat(c);
-      static_cast<T*>(p.dx)[r * D + c] = Tr<T>::from(p.scale * d);
-      static_cast<T*>(p.dh)[r * D + c] = Tr<T>::from(rh * (d * gate(c) * vec<V>(p.w_post, c, 1.f) - b.y - hh * b.x));
-      S1[c] += d * hh;
-      S0[c] += d;
-      T1[c] += dyv(c) * zhat(c);
-      T0[c] += dyv(c);
+  }
+  const int64_t n = p.units * D;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * blockDim.x + threadIdx.x) * VEC;
+    if (c >= D) continue;
+    float* o = p.part + (int64_t)blockIdx.x * D + c;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      o[j] = S1[i][j];
+      o[n + j] = T1[i][j];
+      if (BIAS) o[2 * n + j] = S0[i][j], o[3 * n + j] = T0[i][j];
     }
   }
 }
 
-// The vectors' gradients from the units' sums, one column per thread.
-template <typename V>
-__global__ void __launch_bounds__(NT) finish_kernel(Params p) {
-  const int c = blockIdx.x * NT + threadIdx.x;
-  if (c >= p.dim) return;
+// The vectors' gradients from the units' sums: 32 columns per block, its 32 warps take
+// the groups in turn and are added in order.
+template <bool BIAS>
+__global__ void __launch_bounds__(1024) finish_kernel(Params p) {
+  __shared__ float acc[4][32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
   const int64_t n = p.units * p.dim;
   float w = 0.f, b = 0.f, t1 = 0.f, t0 = 0.f;
-  for (int64_t g = 0; g < p.groups; ++g) {
-    float s1 = 0.f, s0 = 0.f;
-    for (int s = 0; s < p.segs; ++s) {
-      const int64_t at = (g * p.segs + s) * p.dim + c;
-      s1 += p.part[at];
-      s0 += p.part[n + at];
-      t1 += p.part[2 * n + at];
-      t0 += p.part[3 * n + at];
+  if (c < p.dim) {
+    // without a gate per group the units are one run, shared by all warps
+    const int64_t runs = p.groups > 1 ? p.groups : p.segs;
+    const int segs = p.groups > 1 ? p.segs : 1;
+    for (int64_t g = warp; g < runs; g += 32) {
+      float s1 = 0.f, s0 = 0.f;
+      for (int s = 0; s < segs; ++s) {
+        const float* q = p.part + (g * segs + s) * p.dim + c;
+        s1 += q[0];
+        t1 += q[n];
+        if (BIAS) s0 += q[2 * n], t0 += q[3 * n];
+      }
+      if (p.groups > 1) {
+        const float gt = vec1(p.gate, p.vdt, g * p.dim + c, 1.f);
+        w += gt * s1;
+        b += gt * s0;
+        put1(p.dgate, p.vdt, g * p.dim + c,
+             vec1(p.w_post, p.vdt, c, 1.f) * s1 + vec1(p.b_post, p.vdt, c, 0.f) * s0);
+      } else {
+        w += s1;
+        b += s0;
+      }
     }
-    const float gt = vec<V>(p.gate, g * p.dim + c, 1.f);
-    w += gt * s1;
-    b += gt * s0;
-    if (p.dgate)
-      static_cast<V*>(p.dgate)[g * p.dim + c] =
-          Tr<V>::from(vec<V>(p.w_post, c, 1.f) * s1 + vec<V>(p.b_post, c, 0.f) * s0);
   }
-  if (p.dw_post) static_cast<V*>(p.dw_post)[c] = Tr<V>::from(w);
-  if (p.db_post) static_cast<V*>(p.db_post)[c] = Tr<V>::from(b);
-  if (p.dw_pre) static_cast<V*>(p.dw_pre)[c] = Tr<V>::from(t1);
-  if (p.db_pre) static_cast<V*>(p.db_pre)[c] = Tr<V>::from(t0);
+  acc[0][warp][lane] = w;
+  acc[1][warp][lane] = b;
+  acc[2][warp][lane] = t1;
+  acc[3][warp][lane] = t0;
+  __syncthreads();
+  if (warp != 0 || c >= p.dim) return;
+  w = b = t1 = t0 = 0.f;
+  for (int i = 0; i < 32; ++i) {
+    w += acc[0][i][lane];
+    b += acc[1][i][lane];
+    t1 += acc[2][i][lane];
+    t0 += acc[3][i][lane];
+  }
+  if (p.groups <= 1) {
+    if (p.groups == 1) put1(p.dgate, p.vdt, c, vec1(p.w_post, p.vdt, c, 1.f) * w + vec1(p.b_post, p.vdt, c, 0.f) * b);
+    const float gt = p.groups == 1 ? vec1(p.gate, p.vdt, c, 1.f) : 1.f;
+    w *= gt;
+    b *= gt;
+  }
+  put1(p.dw_post, p.vdt, c, w);
+  put1(p.db_post, p.vdt, c, b);
+  put1(p.dw_pre, p.vdt, c, t1);
+  put1(p.db_pre, p.vdt, c, t0);
 }
 
-// Units per group: enough for four blocks on every SM, none without a row.
+// Units per group: about `target` units in all, none without a row.
 static int segments(int64_t rows, int64_t groups) {
   if (groups <= 0 || rows <= 0) return 1;
   const int64_t per = rows / groups;
-  int64_t s = ((int64_t)device_sm_count() * 4 + groups - 1) / groups;
+  int64_t s = ((int64_t)device_sm_count() * 6 + groups - 1) / groups;
   if (s > per) s = per;
   return s < 1 ? 1 : (int)s;
 }
 
-template <typename T, typename V, bool LAYER>
-static void run(const Params& p, bool bwd, cudaStream_t s) {
-  if (!bwd) {
-    forward_kernel<T, V, LAYER><<<(unsigned)p.rows, NT, 0, s>>>(p);
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T, int VEC, int NV, bool WARP>
+static void forward(const Params& p, cudaStream_t s) {
+  if (WARP) {
+    forward_kernel<T, VEC, NV, true><<<(unsigned)((p.rows + 3) / 4), 128, 0, s>>>(p);
   } else {
-    if (p.rows > 0) backward_kernel<T, V, LAYER><<<(unsigned)p.units, NT, 0, s>>>(p);
-    finish_kernel<V><<<(p.dim + NT - 1) / NT, NT, 0, s>>>(p);
+    const int tpr = ((p.dim + VEC * NV - 1) / (VEC * NV) + 31) / 32 * 32;
+    forward_kernel<T, VEC, NV, false><<<(unsigned)p.rows, tpr, 0, s>>>(p);
   }
 }
 
-template <typename T, typename V>
-static void run_kind(int kind, const Params& p, bool bwd, cudaStream_t s) {
-  if (kind == FMS_NORM_LAYER) run<T, V, true>(p, bwd, s);
-  else run<T, V, false>(p, bwd, s);
+template <typename T, int VEC>
+static void run_forward(const Params& p, cudaStream_t s) {
+  constexpr int W = 32 * VEC;  // a warp's columns per run
+  if (p.dim <= W) forward<T, VEC, 1, true>(p, s);
+  else if (p.dim <= 2 * W) forward<T, VEC, 2, true>(p, s);
+  else if (p.dim <= 3 * W) forward<T, VEC, 3, true>(p, s);
+  else if (p.dim <= 4 * W) forward<T, VEC, 4, true>(p, s);
+  else if (VEC > 1 && p.dim <= 1024 * VEC) forward<T, VEC, 1, false>(p, s);
+  else if (p.dim <= 4096 * VEC) forward<T, VEC, 4, false>(p, s);
+  else forward<T, VEC, 16, false>(p, s);
 }
 
-static int launch(int dtype, int vdtype, int kind, const Params& p, bool bwd, cudaStream_t s) {
-  const bool same = dtype == vdtype;
-  if (dtype == FMS_F32) run_kind<float, float>(kind, p, bwd, s);
-  else if (dtype == FMS_F16 && same) run_kind<__half, __half>(kind, p, bwd, s);
-  else if (dtype == FMS_F16) run_kind<__half, float>(kind, p, bwd, s);
-  else if (same) run_kind<__nv_bfloat16, __nv_bfloat16>(kind, p, bwd, s);
-  else run_kind<__nv_bfloat16, float>(kind, p, bwd, s);
+template <typename T, int VEC, int NV, bool BIAS>
+static void backward(const Params& p, cudaStream_t s) {
+  const int tpr = ((p.dim + VEC * NV - 1) / (VEC * NV) + 31) / 32 * 32;
+  backward_kernel<T, VEC, NV, BIAS><<<(unsigned)p.units, tpr, 0, s>>>(p);
+}
+
+template <typename T, int VEC, bool BIAS>
+static void run_backward(const Params& p, cudaStream_t s) {
+  if (VEC > 1) {
+    if (p.dim <= 512 * VEC) backward<T, VEC, 1, BIAS>(p, s);
+    else if (p.dim <= 1024 * VEC) backward<T, VEC, 2, BIAS>(p, s);
+    else backward<T, VEC, VEC == 8 ? 4 : 8, BIAS>(p, s);
+  } else {
+    if (p.dim <= 256) backward<T, VEC, 1, BIAS>(p, s);
+    else if (p.dim <= 2048) backward<T, VEC, 4, BIAS>(p, s);
+    else backward<T, VEC, 32, BIAS>(p, s);
+  }
+}
+
+template <typename T>
+static void run(const Params& p, bool bwd, cudaStream_t s) {
+  constexpr int VEC = 16 / sizeof(T);
+  const bool vec = p.dim % VEC == 0 && aligned16(p.x) && aligned16(p.h) && aligned16(p.w_post) && aligned16(p.b_post) &&
+                   aligned16(p.w_pre) && aligned16(p.b_pre) && aligned16(p.gate) &&
+                   (bwd ? aligned16(p.dz) && aligned16(p.dy) && aligned16(p.dx) && aligned16(p.dh)
+                        : aligned16(p.z) && aligned16(p.y));
+  if (!bwd) {
+    if (vec) run_forward<T, VEC>(p, s);
+    else run_forward<T, 1>(p, s);
+    return;
+  }
+  const bool bias = p.b_post || p.db_post || p.db_pre;
+  if (p.rows > 0) {
+    if (vec && bias) run_backward<T, VEC, true>(p, s);
+    else if (vec) run_backward<T, VEC, false>(p, s);
+    else if (bias) run_backward<T, 1, true>(p, s);
+    else run_backward<T, 1, false>(p, s);
+  }
+  const unsigned blocks = (unsigned)((p.dim + 31) / 32);
+  if (bias) finish_kernel<true><<<blocks, 1024, 0, s>>>(p);
+  else finish_kernel<false><<<blocks, 1024, 0, s>>>(p);
+}
+
+static int launch(int dtype, const Params& p, bool bwd, cudaStream_t s) {
+  if (dtype == FMS_F32) run<float>(p, bwd, s);
+  else if (dtype == FMS_F16) run<__half>(p, bwd, s);
+  else run<__nv_bfloat16>(p, bwd, s);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? FMS_OK : (int)e;
 }
@@ -237,6 +468,7 @@ static int check(int dtype, int vdtype, int kind, int64_t rows, int64_t groups, 
   if (vdtype != dtype && vdtype != FMS_F32) return FMS_ERR_DTYPE;
   if (kind != FMS_NORM_RMS && kind != FMS_NORM_LAYER) return FMS_ERR_INVALID;
   if (rows < 0 || rows > INT32_MAX || dim < 1 || groups < 0 || !(eps >= 0.f)) return FMS_ERR_INVALID;
+  if (dim > FMS_NORM_MAX_DIM) return FMS_ERR_TOO_LARGE;
   if (groups > 0 ? rows % groups != 0 : rows > 0) return FMS_ERR_INVALID;
   return FMS_OK;
 }
@@ -260,7 +492,8 @@ int fms_norm_residual_fwd(int dtype, int vdtype, int kind, const void* x, const 
   p.x = x; p.h = h; p.w_post = w_post; p.b_post = b_post; p.w_pre = w_pre; p.b_pre = b_pre; p.gate = gate;
   p.z = z; p.y = y; p.stats = stats;
   p.rows = rows; p.per = rows / groups; p.dim = dim; p.eps = eps; p.scale = scale;
-  return norm::launch(dtype, vdtype, kind, p, false, (cudaStream_t)stream);
+  p.vdt = vdtype; p.layer = kind == FMS_NORM_LAYER;
+  return norm::launch(dtype, p, false, (cudaStream_t)stream);
 }
 
 size_t fms_norm_residual_bwd_workspace_size(int64_t rows, int64_t groups, int dim) {
@@ -289,7 +522,8 @@ int fms_norm_residual_bwd(int dtype, int vdtype, int kind, const void* x, const 
   p.segs = rows > 0 ? norm::segments(rows, groups) : 0;
   p.units = groups * p.segs;
   p.per = groups > 0 ? rows / groups : 1;
-  return norm::launch(dtype, vdtype, kind, p, true, (cudaStream_t)stream);
+  p.vdt = vdtype; p.layer = kind == FMS_NORM_LAYER;
+  return norm::launch(dtype, p, true, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -21,6 +21,7 @@ from .quant import Int8Index, require_int8_index
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
 NORMS = {"rms": 0, "layer": 1}
+NORM_MAX_DIM = 16384
 _HALF = (torch.float16, torch.bfloat16)
 _FLOAT = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -174,8 +175,8 @@ def norm_residual(x, h, w_post, w_pre, *, gate=None, b_post=None, b_pre=None, sc
     if h.dtype != x.dtype:
         raise ArgumentError("norm_residual: x and h must share an eltype")
     dim = x.shape[-1]
-    if dim < 1:
-        raise DimensionMismatch("norm_residual: feature dim")
+    if not 1 <= dim <= NORM_MAX_DIM:
+        raise DimensionMismatch(f"norm_residual: feature dim must be 1 to {NORM_MAX_DIM}")
     vectors = [v for v in (w_post, w_pre, b_post, b_pre, gate) if v is not None]
     vt = w_post.dtype
     if vt not in (x.dtype, torch.float32) or any(v.dtype != vt for v in vectors):

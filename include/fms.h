@@ -311,8 +311,9 @@ int fms_gated_ffn_bwd(int dtype, const void* x, const void* w_gate, const void* 
    may be NULL.  y is the norm of z before z is rounded.  stats (4, rows) float32,
    when not NULL, keeps the rows' means and reciprocal deviations for the backward
    pass.  Gradient outputs of vectors may be NULL; dz and dy may be NULL (zero).
-   Sums over rows are taken in a fixed order.  Workspace of the backward pass:
+   dim is 1 .. FMS_NORM_MAX_DIM.  Sums over rows are taken in a fixed order.  Workspace of the backward pass:
    fms_norm_residual_bwd_workspace_size. */
+#define FMS_NORM_MAX_DIM 16384
 int fms_norm_residual_fwd(int dtype, int vdtype, int kind, const void* x, const void* h,
                           const void* w_post, const void* b_post, const void* w_pre,
                           const void* b_pre, const void* gate, int64_t groups, int64_t rows, int dim,

@@ -87,7 +87,8 @@ def check(got, ref, t, dz, dy, kind):
 
 
 SHAPES = [(1, 1, 768), (3, 5, 2), (2, 7, 33), (4, 9, 64), (3, 50, 128), (2, 40, 129), (5, 17, 768), (2, 31, 1001),
-          (1, 200, 1024), (2, 3, 2056), (1, 5, 4104), (2, 2, 8200)]
+          (1, 200, 1024), (2, 3, 2056), (1, 5, 4104), (2, 2, 8200), (1, 3, 4099),
+          (1, 2, 9001), (1, 2, 16384)]
 
 
 @pytest.mark.parametrize("kind", ["rms", "layer"])
@@ -266,6 +267,8 @@ def test_refusals(fms):
                       (fms.DimensionMismatch, with_(h=t["h"][:1])),
                       (fms.DimensionMismatch, with_(w_post=t["w_post"][:8])),
                       (fms.DimensionMismatch, with_(gate=t["gate"].expand(3, 16))),
+                      (fms.DimensionMismatch, lambda: fms.norm_residual(*[torch.zeros(n, 16385, device="cuda").squeeze(0)
+                                                                          for n in (2, 2, 1, 1)])),
                       (fms.DimensionMismatch, with_(b_pre=t["b_pre"][None]))]:
         with pytest.raises(err):
             call()
