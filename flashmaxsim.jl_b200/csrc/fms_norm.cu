@@ -20,11 +20,17 @@
 // A group's rows are cut into units, one block each; a unit writes its sums, and a
 // second kernel adds the units in order, so that results repeat bit for bit.
 //
-// All of it is bound by memory: a row is read once into registers (forward x and h,
-// backward x, h, dz and dy) and written once; nothing else but the statistics and the
-// units' sums goes out.
+// All of it is bound by memory: a row is read once (forward x and h, backward x, h, dz
+// and dy) and written once; nothing else but the statistics and the units' sums goes out.
+// What stands in the way is the number of instructions: a row of 768 leaves an SM 270
+// (forward) and 400 (backward) cycles of memory time.  So the arithmetic is in pairs
+// (f32x2), and rows are read straight into registers: a ring of bulk copies was slower
+// (forward 112 us against 103 at 46080 x 768, the thread that issues them holds up its
+// row).
 #include "fms_common.cuh"
 #include "fms_internal.h"
+
+#include <type_traits>
 
 namespace fms {
 namespace norm {
@@ -43,58 +49,96 @@ struct Params {
   float eps, scale;
 };
 
-// VEC neighbouring values as float32: one 16-byte access, or one value (rows that do not
-// start on 16 bytes).
-template <typename T, int VEC>
-__device__ __forceinline__ void load(const T* p, float (&f)[VEC]) {
-  if constexpr (VEC == 1) {
-    f[0] = Tr<T>::to(*p);
-  } else {
-    const uint4 q = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+// A thread's values of a row: N pairs, in runs of VEC neighbours (one 16-byte access
+// each; VEC 1 for rows that do not start on 16 bytes), run i at (i * tpr + tid) * VEC.
+// `raw` holds them as they lie in memory.
+template <typename T, int VEC, int N>
+struct Raw {
+  static constexpr int RUNS = 2 * N / VEC;
+  using Word = typename std::conditional<VEC == 1, T, uint4>::type;
+  Word w[RUNS];
+  __device__ __forceinline__ void load(const T* row, int tid, int tpr, int D) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (sizeof(T) == 4) {
-        f[j] = __uint_as_float(w[j]);
-      } else {
-        const T* t = reinterpret_cast<const T*>(&w[j]);
-        f[2 * j] = Tr<T>::to(t[0]);
-        f[2 * j + 1] = Tr<T>::to(t[1]);
+    for (int i = 0; i < RUNS; ++i) {
+      const int c = (i * tpr + tid) * VEC;
+      if constexpr (VEC == 1) w[i] = c < D ? row[c] : Tr<T>::from(0.f);
+      else w[i] = c < D ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void get(float2 (&f)[N]) const {
+    if constexpr (VEC == 1) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) f[k] = make_float2(Tr<T>::to(w[2 * k]), Tr<T>::to(w[2 * k + 1]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i) {
+        const uint32_t q[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+        for (int k = 0; k < VEC / 2; ++k) f[i * (VEC / 2) + k] = pair(q, k);
       }
     }
   }
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void store(T* p, const float (&f)[VEC]) {
-  if constexpr (VEC == 1) {
-    *p = Tr<T>::from(f[0]);
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (sizeof(T) == 4) {
-        w[j] = __float_as_uint(f[j]);
-      } else {
-        T t[2] = {Tr<T>::from(f[2 * j]), Tr<T>::from(f[2 * j + 1])};
-        w[j] = *reinterpret_cast<const uint32_t*>(t);
-      }
+  static __device__ __forceinline__ float2 pair(const uint32_t (&q)[4], int k) {
+    if constexpr (sizeof(T) == 4) {
+      return make_float2(__uint_as_float(q[2 * (k & 1)]), __uint_as_float(q[2 * (k & 1) + 1]));
+    } else if constexpr (std::is_same<T, __half>::value) {
+      return __half22float2(*reinterpret_cast<const __half2*>(&q[k]));
+    } else {
+      return make_float2(__uint_as_float(q[k] << 16), __uint_as_float(q[k] & 0xffff0000u));
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// The pairs of one run written to a row.
+template <typename T, int VEC, int N>
+__device__ __forceinline__ void store(T* row, int tid, int tpr, int D, const float2 (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < 2 * N / VEC; ++i) {
+    const int c = (i * tpr + tid) * VEC;
+    if (c >= D) continue;
+    if constexpr (VEC == 1) {
+      row[c] = Tr<T>::from(i & 1 ? f[i >> 1].y : f[i >> 1].x);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) {
+          w[j] = __float_as_uint(j & 1 ? f[i * 2 + (j >> 1)].y : f[i * 2 + (j >> 1)].x);
+        } else {
+          const float2 v = f[i * 4 + j];
+          if constexpr (std::is_same<T, __half>::value) {
+            const __half2 h = __floats2half2_rn(v.x, v.y);
+            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+          } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+        }
+      }
+      *reinterpret_cast<uint4*>(row + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
 }
-// The same of a weight, bias or gate (in T or float32); `none` where there is none.
-template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const void* p, int vdt, int64_t at, float none, float (&f)[VEC]) {
-  if (p == nullptr) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) f[j] = none;
-  } else if (vdt == FMS_F32) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) f[j] = __ldg(static_cast<const float*>(p) + at + j);
+
+// The same of a weight, bias or gate (in T or float32) from element `at` on.
+template <typename T, int VEC, int N>
+__device__ __forceinline__ void load_vec(const void* p, int vdt, int64_t at, int tid, int tpr, int D, float2 (&f)[N]) {
+  if (sizeof(T) == 4 || vdt != FMS_F32) {
+    Raw<T, VEC, N> r;
+    r.load(static_cast<const T*>(p) + at, tid, tpr, D);
+    r.get(f);
   } else {
-    load<T, VEC>(static_cast<const T*>(p) + at, f);
+    const float* q = static_cast<const float*>(p) + at;
+#pragma unroll
+    for (int e = 0; e < 2 * N; ++e) {
+      const int c = (e / VEC * tpr + tid) * VEC + e % VEC;
+      const float v = c < D ? __ldg(q + c) : 0.f;
+      if (e & 1) f[e >> 1].y = v;
+      else f[e >> 1].x = v;
+    }
   }
 }
+__device__ __forceinline__ float2 two(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float vec1(const void* p, int vdt, int64_t i, float none) {
   if (p == nullptr) return none;
   return vdt == FMS_F32   ? static_cast<const float*>(p)[i]
@@ -110,102 +154,108 @@ __device__ __forceinline__ void put1(void* p, int vdt, int64_t i, float v) {
 
 constexpr int MAX_WARPS = 32;
 
-// Sums of two values over the threads of a row, the same on each of them: a warp, or
-// the whole block (one barrier: the partial sums alternate between two places).
-template <bool WARP>
+// Sums of N values over the threads of a row, the same on each of them: a warp, or the
+// whole block (one barrier: the partial sums alternate between two places).
+template <bool WARP, int N>
 struct RowSum {
-  float2 (*part)[MAX_WARPS];
+  float (*part)[MAX_WARPS * N];
   int turn = 0;
-  __device__ __forceinline__ float2 operator()(float2 v) {
+  __device__ __forceinline__ void operator()(float (&v)[N]) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+    if (WARP) return;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) part[turn][(threadIdx.x >> 5) * N + k] = v[k];
     }
-    if (WARP) return v;
-    if ((threadIdx.x & 31) == 0) part[turn][threadIdx.x >> 5] = v;
     __syncthreads();
     const int n = blockDim.x >> 5;
-    float2 t = part[turn][0];
-    for (int i = 1; i < n; ++i) t.x += part[turn][i].x, t.y += part[turn][i].y;
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = part[turn][k];
+    for (int i = 1; i < n; ++i)
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] += part[turn][i * N + k];
     turn ^= 1;
-    return t;
   }
 };
 
-// One row per warp (WARP) or block; a thread holds NV runs of VEC values.  A warp takes
-// rows of up to 4 runs per lane (no barriers between the row's sums), a block the wider
-// ones.
-template <typename T, int VEC, int NV, bool WARP>
+// One row per warp (WARP, rows of up to 1024) or block; a thread holds N pairs.
+template <typename T, int VEC, int N, bool WARP>
 __global__ void __launch_bounds__(WARP ? 128 : 1024) forward_kernel(Params p) {
-  __shared__ float2 part[2][MAX_WARPS];
-  RowSum<WARP> sum{part};
+  __shared__ float part[2][MAX_WARPS];
+  RowSum<WARP, 1> sum{part};
   const int64_t r = WARP ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
   if (WARP && r >= p.rows) return;
   const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, tpr = WARP ? 32 : blockDim.x;
   const int D = p.dim;
   const float inv_d = 1.f / D;
-  const T* x = static_cast<const T*>(p.x) + r * D;
-  const T* h = static_cast<const T*>(p.h) + r * D;
-  const int64_t g0 = (r / p.per) * D;
-  float z[NV][VEC], v[NV][VEC];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * tpr + tid) * VEC;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) z[i][j] = v[i][j] = 0.f;
-    if (c < D) {
-      load<T, VEC>(h + c, v[i]);
-      load<T, VEC>(x + c, z[i]);
-    }
+  float2 z[N], v[N], w[N];
+  {
+    Raw<T, VEC, N> h, x;
+    h.load(static_cast<const T*>(p.h) + r * D, tid, tpr, D);
+    x.load(static_cast<const T*>(p.x) + r * D, tid, tpr, D);
+    h.get(v);
+    x.get(z);
   }
   // mean, and the reciprocal deviation of the centred values (two passes over registers)
-  auto stats = [&](float (&a)[NV][VEC], float& mean, float& rstd) {
+  auto stats = [&](float2 (&a)[N], float& mean, float& rstd) {
+    float s[1];
     mean = 0.f;
     if (p.layer) {
-      float s = 0.f;
+      float2 t = a[0];
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s += a[i][j];
-      mean = sum({s, 0.f}).x * inv_d;
+      for (int k = 1; k < N; ++k) t = __fadd2_rn(t, a[k]);
+      s[0] = t.x + t.y;
+      sum(s);
+      mean = s[0] * inv_d;
     }
-    float s = 0.f;
+    float2 t = two(0.f);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < 2 * N / VEC; ++i)
+      if ((i * tpr + tid) * VEC < D) {  // the values past the row's end are no zeros once centred
+        if constexpr (VEC == 1) {
+          const float d = (i & 1 ? a[i >> 1].y : a[i >> 1].x) - mean;
+          t.x = fmaf(d, d, t.x);
+        } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float d = (i * tpr + tid) * VEC < D ? a[i][j] - mean : 0.f;
-        s += d * d;
+          for (int k = 0; k < VEC / 2; ++k) {
+            const float2 d = __fadd2_rn(a[i * (VEC / 2) + k], two(-mean));
+            t = __ffma2_rn(d, d, t);
+          }
+        }
       }
-    rstd = rsqrtf(sum({s, 0.f}).x * inv_d + p.eps);
+    s[0] = t.x + t.y;
+    sum(s);
+    rstd = rsqrtf(s[0] * inv_d + p.eps);
+  };
+  // v = (a - mean) rstd w + b
+  auto apply = [&](float2 (&a)[N], float mean, float rstd, const void* wv, const void* bv) {
+    load_vec<T, VEC, N>(wv, p.vdt, 0, tid, tpr, D, w);
+    const float shift = -mean * rstd;
+#pragma unroll
+    for (int k = 0; k < N; ++k) a[k] = __fmul2_rn(__ffma2_rn(a[k], two(rstd), two(shift)), w[k]);
+    if (bv) {
+      load_vec<T, VEC, N>(bv, p.vdt, 0, tid, tpr, D, w);
+#pragma unroll
+      for (int k = 0; k < N; ++k) a[k] = __fadd2_rn(a[k], w[k]);
+    }
   };
   float mh, rh, mz, rz;
   stats(v, mh, rh);
+  apply(v, mh, rh, p.w_post, p.b_post);
+  if (p.gate) {
+    load_vec<T, VEC, N>(p.gate, p.vdt, (r / p.per) * D, tid, tpr, D, w);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * tpr + tid) * VEC;
-    if (c >= D) continue;
-    float w[VEC], b[VEC], g[VEC];
-    load_vec<T, VEC>(p.w_post, p.vdt, c, 1.f, w);
-    load_vec<T, VEC>(p.b_post, p.vdt, c, 0.f, b);
-    load_vec<T, VEC>(p.gate, p.vdt, g0 + c, 1.f, g);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) z[i][j] = p.scale * z[i][j] + g[j] * ((v[i][j] - mh) * rh * w[j] + b[j]);
-    store<T, VEC>(static_cast<T*>(p.z) + r * D + c, z[i]);
+    for (int k = 0; k < N; ++k) v[k] = __fmul2_rn(v[k], w[k]);
   }
+#pragma unroll
+  for (int k = 0; k < N; ++k) z[k] = __ffma2_rn(z[k], two(p.scale), v[k]);
+  store<T, VEC, N>(static_cast<T*>(p.z) + r * D, tid, tpr, D, z);
   stats(z, mz, rz);
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * tpr + tid) * VEC;
-    if (c >= D) continue;
-    float w[VEC], b[VEC];
-    load_vec<T, VEC>(p.w_pre, p.vdt, c, 1.f, w);
-    load_vec<T, VEC>(p.b_pre, p.vdt, c, 0.f, b);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) z[i][j] = (z[i][j] - mz) * rz * w[j] + b[j];
-    store<T, VEC>(static_cast<T*>(p.y) + r * D + c, z[i]);
-  }
+  apply(z, mz, rz, p.w_pre, p.b_pre);
+  store<T, VEC, N>(static_cast<T*>(p.y) + r * D, tid, tpr, D, z);
   if (p.stats && tid == 0) {
     p.stats[r] = mh;
     p.stats[p.rows + r] = rh;
@@ -214,127 +264,117 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) forward_kernel(Params p) {
   }
 }
 
-// One unit (a run of one group's rows) per block, a row at a time; a thread owns the
-// same NV runs of VEC columns in every row and keeps their sums in registers.  BIAS:
-// S0 and T0 are wanted too.
-template <typename T, int VEC, int NV, bool BIAS>
+// One unit (a run of one group's rows) per block, a row at a time with the next one's
+// loads in flight; a thread owns the same N pairs of columns in every row and keeps
+// their sums in registers.  BIAS: S0 and T0 are wanted too.
+template <typename T, int VEC, int N, bool BIAS>
 __global__ void __launch_bounds__(512) backward_kernel(Params p) {
-  __shared__ float2 part[2][MAX_WARPS];
-  RowSum<false> sum{part};
-  const int D = p.dim;
+  __shared__ float part[2][MAX_WARPS * 2];
+  RowSum<false, 2> sum{part};
+  const int D = p.dim, tid = threadIdx.x, tpr = blockDim.x;
   const float inv_d = 1.f / D;
   const int64_t group = blockIdx.x / p.segs, seg = blockIdx.x % p.segs;
   const int64_t r0 = group * p.per + p.per * seg / p.segs, r1 = group * p.per + p.per * (seg + 1) / p.segs;
-  float gw[NV][VEC], gb[NV][VEC], wp[NV][VEC];  // gate w_post, gate b_post, w_pre
-  float S1[NV][VEC], T1[NV][VEC], S0[NV][VEC], T0[NV][VEC];
+  float2 gw[N], gb[N], wp[N];  // gate w_post, gate b_post, w_pre
+  float2 S1[N], T1[N], S0[N], T0[N];
+  load_vec<T, VEC, N>(p.w_post, p.vdt, 0, tid, tpr, D, gw);
+  load_vec<T, VEC, N>(p.w_pre, p.vdt, 0, tid, tpr, D, wp);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * VEC;
-    float g[VEC];
+  for (int k = 0; k < N; ++k) S1[k] = T1[k] = S0[k] = T0[k] = gb[k] = two(0.f);
+  if (BIAS && p.b_post) load_vec<T, VEC, N>(p.b_post, p.vdt, 0, tid, tpr, D, gb);
+  if (p.gate) {
+    float2 g[N];
+    load_vec<T, VEC, N>(p.gate, p.vdt, group * D, tid, tpr, D, g);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      S1[i][j] = T1[i][j] = S0[i][j] = T0[i][j] = 0.f;
-      gw[i][j] = gb[i][j] = wp[i][j] = g[j] = 0.f;
-    }
-    if (c >= D) continue;
-    load_vec<T, VEC>(p.gate, p.vdt, group * D + c, 1.f, g);
-    load_vec<T, VEC>(p.w_post, p.vdt, c, 1.f, gw[i]);
-    if (BIAS) load_vec<T, VEC>(p.b_post, p.vdt, c, 0.f, gb[i]);
-    load_vec<T, VEC>(p.w_pre, p.vdt, c, 1.f, wp[i]);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) gw[i][j] *= g[j], gb[i][j] *= g[j];
+    for (int k = 0; k < N; ++k) gw[k] = __fmul2_rn(gw[k], g[k]), gb[k] = __fmul2_rn(gb[k], g[k]);
   }
+  Raw<T, VEC, N> rx, rhh, ry, rd;
+  float st[4];
+  auto fetch = [&](int64_t r) {
+    rx.load(static_cast<const T*>(p.x) + r * D, tid, tpr, D);
+    rhh.load(static_cast<const T*>(p.h) + r * D, tid, tpr, D);
+    if (p.dy) ry.load(static_cast<const T*>(p.dy) + r * D, tid, tpr, D);
+    if (p.dz) rd.load(static_cast<const T*>(p.dz) + r * D, tid, tpr, D);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) st[k] = __ldg(p.stats + k * p.rows + r);
+  };
+  fetch(r0);
   for (int64_t r = r0; r < r1; ++r) {
-    const float mh = p.stats[r], rh = p.stats[p.rows + r], mz = p.stats[2 * p.rows + r], rz = p.stats[3 * p.rows + r];
-    float hh[NV][VEC], zh[NV][VEC], dy[NV][VEC], d[NV][VEC];
-    float2 a = {0.f, 0.f};
+    const float mh = st[0], rh = st[1], mz = st[2], rz = st[3];
+    float2 hh[N], zh[N], dy[N], d[N];
+    rx.get(zh);
+    rhh.get(hh);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * VEC;
-      const int64_t at = r * D + c;
+    for (int k = 0; k < N; ++k) dy[k] = d[k] = two(0.f);
+    if (p.dy) ry.get(dy);
+    if (p.dz) rd.get(d);
+    if (r + 1 < r1) fetch(r + 1);
+    const float2 nh = two(-mh * rh), nz = two(-mz * rz);
+    float2 s0 = two(0.f), s1 = two(0.f);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) hh[i][j] = zh[i][j] = dy[i][j] = d[i][j] = 0.f;
-      if (c >= D) continue;
-      load<T, VEC>(static_cast<const T*>(p.x) + at, zh[i]);
-      load<T, VEC>(static_cast<const T*>(p.h) + at, hh[i]);
-      if (p.dy) load<T, VEC>(static_cast<const T*>(p.dy) + at, dy[i]);
-      if (p.dz) load<T, VEC>(static_cast<const T*>(p.dz) + at, d[i]);
+    for (int k = 0; k < N; ++k) {
+      hh[k] = __ffma2_rn(hh[k], two(rh), nh);
+      float2 z = __ffma2_rn(hh[k], gw[k], __fmul2_rn(zh[k], two(p.scale)));
+      if (BIAS) z = __fadd2_rn(z, gb[k]);
+      zh[k] = __ffma2_rn(z, two(rz), nz);
+      const float2 t = __fmul2_rn(dy[k], wp[k]);  // 0 past the row's end
+      s0 = __ffma2_rn(t, zh[k], s0);
+      s1 = __fadd2_rn(s1, t);
     }
+    float a[2] = {s0.x + s0.y, s1.x + s1.y};
+    sum(a);
+    const float2 ka = two(-rz * a[0] * inv_d), km = two(p.layer ? -rz * a[1] * inv_d : 0.f);
+    s0 = s1 = two(0.f);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if ((i * (int)blockDim.x + (int)threadIdx.x) * VEC >= D) continue;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        hh[i][j] = (hh[i][j] - mh) * rh;
-        zh[i][j] = (p.scale * zh[i][j] + (hh[i][j] * gw[i][j] + gb[i][j]) - mz) * rz;
-        const float t = dy[i][j] * wp[i][j];
-        a.x += t * zh[i][j];
-        a.y += t;
-      }
+    for (int k = 0; k < N; ++k) {
+      d[k] = __ffma2_rn(__fmul2_rn(dy[k], wp[k]), two(rz), __fadd2_rn(d[k], km));
+      d[k] = __ffma2_rn(zh[k], ka, d[k]);
+      const float2 e = __fmul2_rn(d[k], gw[k]);  // 0 past the row's end
+      s0 = __ffma2_rn(e, hh[k], s0);
+      s1 = __fadd2_rn(s1, e);
     }
-    a = sum(a);
-    a.x *= inv_d;
-    a.y = p.layer ? a.y * inv_d : 0.f;
-    float2 b = {0.f, 0.f};
+    float b[2] = {s0.x + s0.y, s1.x + s1.y};
+    sum(b);
+    const float2 kb = two(-rh * b[0] * inv_d), kn = two(p.layer ? -rh * b[1] * inv_d : 0.f);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        d[i][j] += rz * (dy[i][j] * wp[i][j] - a.y - zh[i][j] * a.x);
-        const float e = d[i][j] * gw[i][j];  // 0 past the row's end
-        b.x += e * hh[i][j];
-        b.y += e;
-      }
-    b = sum(b);
-    b.x *= inv_d;
-    b.y = p.layer ? b.y * inv_d : 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * VEC;
-      if (c >= D) continue;
-      const int64_t at = r * D + c;
-      float o[VEC], q[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        o[j] = p.scale * d[i][j];
-        q[j] = rh * (d[i][j] * gw[i][j] - b.y - hh[i][j] * b.x);
-        S1[i][j] += d[i][j] * hh[i][j];
-        T1[i][j] += dy[i][j] * zh[i][j];
-        if (BIAS) S0[i][j] += d[i][j], T0[i][j] += dy[i][j];
-      }
-      store<T, VEC>(static_cast<T*>(p.dx) + at, o);
-      store<T, VEC>(static_cast<T*>(p.dh) + at, q);
+    for (int k = 0; k < N; ++k) {
+      S1[k] = __ffma2_rn(d[k], hh[k], S1[k]);
+      T1[k] = __ffma2_rn(dy[k], zh[k], T1[k]);
+      if (BIAS) S0[k] = __fadd2_rn(S0[k], d[k]), T0[k] = __fadd2_rn(T0[k], dy[k]);
+      const float2 e = __fmul2_rn(d[k], gw[k]);
+      hh[k] = __ffma2_rn(hh[k], kb, __ffma2_rn(e, two(rh), kn));
+      d[k] = __fmul2_rn(d[k], two(p.scale));
     }
+    store<T, VEC, N>(static_cast<T*>(p.dx) + r * D, tid, tpr, D, d);
+    store<T, VEC, N>(static_cast<T*>(p.dh) + r * D, tid, tpr, D, hh);
   }
   const int64_t n = p.units * D;
+  float* o = p.part + (int64_t)blockIdx.x * D;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * VEC;
+  for (int e = 0; e < 2 * N; ++e) {
+    const int c = (e / VEC * tpr + tid) * VEC + e % VEC, k = e >> 1;
     if (c >= D) continue;
-    float* o = p.part + (int64_t)blockIdx.x * D + c;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      o[j] = S1[i][j];
-      o[n + j] = T1[i][j];
-      if (BIAS) o[2 * n + j] = S0[i][j], o[3 * n + j] = T0[i][j];
-    }
+    o[c] = e & 1 ? S1[k].y : S1[k].x;
+    o[n + c] = e & 1 ? T1[k].y : T1[k].x;
+    if (BIAS) o[2 * n + c] = e & 1 ? S0[k].y : S0[k].x, o[3 * n + c] = e & 1 ? T0[k].y : T0[k].x;
   }
 }
 
-// The vectors' gradients from the units' sums: 32 columns per block, its 32 warps take
-// the groups in turn and are added in order.
+// The vectors' gradients from the units' sums, in two steps.  First, 32 columns per block:
+// part blockIdx.y of the groups (of the units, where there is one group), its 32 warps in
+// turn, added in order; the gates' gradients are complete here.
 template <bool BIAS>
-__global__ void __launch_bounds__(1024) finish_kernel(Params p) {
+__global__ void __launch_bounds__(1024) gather_kernel(Params p, float* out) {
   __shared__ float acc[4][32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   const int64_t n = p.units * p.dim;
+  const bool many = p.groups > 1;
+  const int64_t runs = many ? p.groups : p.segs;
+  const int segs = many ? p.segs : 1;
   float w = 0.f, b = 0.f, t1 = 0.f, t0 = 0.f;
   if (c < p.dim) {
-    // without a gate per group the units are one run, shared by all warps
-    const int64_t runs = p.groups > 1 ? p.groups : p.segs;
-    const int segs = p.groups > 1 ? p.segs : 1;
-    for (int64_t g = warp; g < runs; g += 32) {
+    for (int64_t g = (int64_t)blockIdx.y * 32 + warp; g < runs; g += gridDim.y * 32) {
       float s1 = 0.f, s0 = 0.f;
       for (int s = 0; s < segs; ++s) {
         const float* q = p.part + (g * segs + s) * p.dim + c;
@@ -342,16 +382,12 @@ __global__ void __launch_bounds__(1024) finish_kernel(Params p) {
         t1 += q[n];
         if (BIAS) s0 += q[2 * n], t0 += q[3 * n];
       }
-      if (p.groups > 1) {
-        const float gt = vec1(p.gate, p.vdt, g * p.dim + c, 1.f);
-        w += gt * s1;
-        b += gt * s0;
+      const float gt = many ? vec1(p.gate, p.vdt, g * p.dim + c, 1.f) : 1.f;
+      w += gt * s1;
+      b += gt * s0;
+      if (many)
         put1(p.dgate, p.vdt, g * p.dim + c,
              vec1(p.w_post, p.vdt, c, 1.f) * s1 + vec1(p.b_post, p.vdt, c, 0.f) * s0);
-      } else {
-        w += s1;
-        b += s0;
-      }
     }
   }
   acc[0][warp][lane] = w;
@@ -359,76 +395,80 @@ __global__ void __launch_bounds__(1024) finish_kernel(Params p) {
   acc[2][warp][lane] = t1;
   acc[3][warp][lane] = t0;
   __syncthreads();
-  if (warp != 0 || c >= p.dim) return;
-  w = b = t1 = t0 = 0.f;
-  for (int i = 0; i < 32; ++i) {
-    w += acc[0][i][lane];
-    b += acc[1][i][lane];
-    t1 += acc[2][i][lane];
-    t0 += acc[3][i][lane];
+  if (warp >= 4 || c >= p.dim) return;
+  float s = 0.f;
+  for (int i = 0; i < 32; ++i) s += acc[warp][i][lane];
+  out[((int64_t)blockIdx.y * 4 + warp) * p.dim + c] = s;
+}
+
+__global__ void __launch_bounds__(128) finish_kernel(Params p, const float* in, int parts) {
+  const int c = blockIdx.x * 128 + threadIdx.x;
+  if (c >= p.dim) return;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < parts; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[k] += in[((int64_t)i * 4 + k) * p.dim + c];
+  if (p.groups == 1) {
+    put1(p.dgate, p.vdt, c, vec1(p.w_post, p.vdt, c, 1.f) * s[0] + vec1(p.b_post, p.vdt, c, 0.f) * s[1]);
+    const float gt = vec1(p.gate, p.vdt, c, 1.f);
+    s[0] *= gt;
+    s[1] *= gt;
   }
-  if (p.groups <= 1) {
-    if (p.groups == 1) put1(p.dgate, p.vdt, c, vec1(p.w_post, p.vdt, c, 1.f) * w + vec1(p.b_post, p.vdt, c, 0.f) * b);
-    const float gt = p.groups == 1 ? vec1(p.gate, p.vdt, c, 1.f) : 1.f;
-    w *= gt;
-    b *= gt;
-  }
-  put1(p.dw_post, p.vdt, c, w);
-  put1(p.db_post, p.vdt, c, b);
-  put1(p.dw_pre, p.vdt, c, t1);
-  put1(p.db_pre, p.vdt, c, t0);
+  put1(p.dw_post, p.vdt, c, s[0]);
+  put1(p.db_post, p.vdt, c, s[1]);
+  put1(p.dw_pre, p.vdt, c, s[2]);
+  put1(p.db_pre, p.vdt, c, s[3]);
+}
+
+constexpr int MAX_PARTS = 16;
+static int parts_of(int64_t groups, int segs) {
+  const int64_t runs = groups > 1 ? groups : segs;
+  int64_t n = (runs + 31) / 32;
+  return n < 1 ? 1 : n > MAX_PARTS ? MAX_PARTS : (int)n;
 }
 
 // Units per group: about `target` units in all, none without a row.
 static int segments(int64_t rows, int64_t groups) {
   if (groups <= 0 || rows <= 0) return 1;
   const int64_t per = rows / groups;
-  int64_t s = ((int64_t)device_sm_count() * 6 + groups - 1) / groups;
+  int64_t s = (int64_t)device_sm_count() * 5 / groups;
   if (s > per) s = per;
   return s < 1 ? 1 : (int)s;
 }
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <typename T, int VEC, int NV, bool WARP>
+template <typename T, int VEC, int N, bool WARP>
 static void forward(const Params& p, cudaStream_t s) {
-  if (WARP) {
-    forward_kernel<T, VEC, NV, true><<<(unsigned)((p.rows + 3) / 4), 128, 0, s>>>(p);
+  if constexpr (WARP) {
+    forward_kernel<T, VEC, N, true><<<(unsigned)((p.rows + 3) / 4), 128, 0, s>>>(p);
   } else {
-    const int tpr = ((p.dim + VEC * NV - 1) / (VEC * NV) + 31) / 32 * 32;
-    forward_kernel<T, VEC, NV, false><<<(unsigned)p.rows, tpr, 0, s>>>(p);
+    const int tpr = (p.dim + 2 * N * 32 - 1) / (2 * N * 32) * 32;
+    forward_kernel<T, VEC, N, false><<<(unsigned)p.rows, tpr, 0, s>>>(p);
   }
 }
 
 template <typename T, int VEC>
 static void run_forward(const Params& p, cudaStream_t s) {
-  constexpr int W = 32 * VEC;  // a warp's columns per run
-  if (p.dim <= W) forward<T, VEC, 1, true>(p, s);
-  else if (p.dim <= 2 * W) forward<T, VEC, 2, true>(p, s);
-  else if (p.dim <= 3 * W) forward<T, VEC, 3, true>(p, s);
-  else if (p.dim <= 4 * W) forward<T, VEC, 4, true>(p, s);
-  else if (VEC > 1 && p.dim <= 1024 * VEC) forward<T, VEC, 1, false>(p, s);
-  else if (p.dim <= 4096 * VEC) forward<T, VEC, 4, false>(p, s);
-  else forward<T, VEC, 16, false>(p, s);
+  if (p.dim <= 256) forward<T, VEC, 4, true>(p, s);
+  else if (p.dim <= 512) forward<T, VEC, 8, true>(p, s);
+  else if (p.dim <= 768) forward<T, VEC, 12, true>(p, s);
+  else if (p.dim <= 1024) forward<T, VEC, 16, true>(p, s);
+  else if (p.dim <= 8192) forward<T, VEC, 4, false>(p, s);
+  else forward<T, VEC, 8, false>(p, s);
 }
 
-template <typename T, int VEC, int NV, bool BIAS>
+template <typename T, int VEC, int N, bool BIAS>
 static void backward(const Params& p, cudaStream_t s) {
-  const int tpr = ((p.dim + VEC * NV - 1) / (VEC * NV) + 31) / 32 * 32;
-  backward_kernel<T, VEC, NV, BIAS><<<(unsigned)p.units, tpr, 0, s>>>(p);
+  const int tpr = (p.dim + 2 * N * 32 - 1) / (2 * N * 32) * 32;
+  backward_kernel<T, VEC, N, BIAS><<<(unsigned)p.units, tpr, 0, s>>>(p);
 }
 
 template <typename T, int VEC, bool BIAS>
 static void run_backward(const Params& p, cudaStream_t s) {
-  if (VEC > 1) {
-    if (p.dim <= 512 * VEC) backward<T, VEC, 1, BIAS>(p, s);
-    else if (p.dim <= 1024 * VEC) backward<T, VEC, 2, BIAS>(p, s);
-    else backward<T, VEC, VEC == 8 ? 4 : 8, BIAS>(p, s);
-  } else {
-    if (p.dim <= 256) backward<T, VEC, 1, BIAS>(p, s);
-    else if (p.dim <= 2048) backward<T, VEC, 4, BIAS>(p, s);
-    else backward<T, VEC, 32, BIAS>(p, s);
-  }
+  if (p.dim <= 4096) backward<T, VEC, 4, BIAS>(p, s);
+  else if (p.dim <= 8192) backward<T, VEC, 8, BIAS>(p, s);
+  else backward<T, VEC, 16, BIAS>(p, s);
 }
 
 template <typename T>
@@ -450,9 +490,12 @@ static void run(const Params& p, bool bwd, cudaStream_t s) {
     else if (bias) run_backward<T, 1, true>(p, s);
     else run_backward<T, 1, false>(p, s);
   }
-  const unsigned blocks = (unsigned)((p.dim + 31) / 32);
-  if (bias) finish_kernel<true><<<blocks, 1024, 0, s>>>(p);
-  else finish_kernel<false><<<blocks, 1024, 0, s>>>(p);
+  const int parts = parts_of(p.groups, p.segs);
+  float* sums = p.part + 4 * p.units * p.dim;
+  const dim3 grid((unsigned)((p.dim + 31) / 32), (unsigned)parts);
+  if (bias) gather_kernel<true><<<grid, 1024, 0, s>>>(p, sums);
+  else gather_kernel<false><<<grid, 1024, 0, s>>>(p, sums);
+  finish_kernel<<<(unsigned)((p.dim + 127) / 128), 128, 0, s>>>(p, sums, parts);
 }
 
 static int launch(int dtype, const Params& p, bool bwd, cudaStream_t s) {
@@ -474,6 +517,7 @@ static int check(int dtype, int vdtype, int kind, int64_t rows, int64_t groups, 
 }
 
 }  // namespace norm
+
 }  // namespace fms
 
 using namespace fms;
@@ -497,8 +541,9 @@ int fms_norm_residual_fwd(int dtype, int vdtype, int kind, const void* x, const 
 }
 
 size_t fms_norm_residual_bwd_workspace_size(int64_t rows, int64_t groups, int dim) {
-  if (rows <= 0 || groups <= 0 || dim <= 0) return 0;
-  return (size_t)4 * groups * norm::segments(rows, groups) * dim * sizeof(float);
+  if (rows < 0 || groups < 0 || dim <= 0) return 0;
+  const int segs = rows > 0 ? norm::segments(rows, groups) : 0;
+  return ((size_t)groups * segs + norm::parts_of(groups, segs)) * 4 * dim * sizeof(float);
 }
 
 int fms_norm_residual_bwd(int dtype, int vdtype, int kind, const void* x, const void* h, const void* w_post,
