@@ -17,11 +17,12 @@
 // T1 = sum dy zhat, T0 = sum dy, from which every vector's gradient follows:
 //   dw_post = sum_g gate S1, db_post = sum_g gate S0, dw_pre = sum T1,
 //   db_pre = sum T0, dgate = w_post S1 + b_post S0.
-// A group's rows are cut into units, one block each; a unit writes its sums, and a
-// second kernel adds the units in order, so that results repeat bit for bit.
+// Each block takes an equal run of the rows, whatever groups they belong to, and writes
+// S for every group that it meets and T once; two small kernels add these in order, so
+// that results repeat bit for bit.
 //
 // All of it is bound by memory: a row is read once (forward x and h, backward x, h, dz
-// and dy) and written once; nothing else but the statistics and the units' sums goes out.
+// and dy) and written once; nothing else but the statistics and the blocks' sums goes out.
 // What stands in the way is the number of instructions: a row of 768 leaves an SM 270
 // (forward) and 400 (backward) cycles of memory time.  So the arithmetic is in pairs
 // (f32x2), and rows are read straight into registers: a ring of bulk copies was slower
@@ -41,10 +42,9 @@ struct Params {
   void *z, *y, *dx, *dh;              // rows in T
   void *dw_post, *db_post, *dw_pre, *db_pre, *dgate;   // vectors in vdt, or NULL
   float* stats;                       // (4, rows): mean and rstd of h, mean and rstd of z
-  float* part;                        // (4, units, dim): S1, T1, S0, T0
+  float* part;                        // S1, S0: (blocks + groups, dim); T1, T0: (blocks, dim)
   int64_t rows, per, groups;          // rows per gate vector, gate vectors
-  int64_t units;                      // units of the backward pass
-  int segs;                           // units per group (0 without rows)
+  int64_t blocks;                     // of the backward pass (0 without rows)
   int dim, vdt, layer;
   float eps, scale;
 };
@@ -264,30 +264,53 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) forward_kernel(Params p) {
   }
 }
 
-// One unit (a run of one group's rows) per block, a row at a time with the next one's
-// loads in flight; a thread owns the same N pairs of columns in every row and keeps
-// their sums in registers.  BIAS: S0 and T0 are wanted too.
+// Block k's rows start at rows k / blocks; the block that holds row r.
+__device__ __forceinline__ int64_t block_of(const Params& p, int64_t r) { return ((r + 1) * p.blocks - 1) / p.rows; }
+
+template <int VEC, int N>
+__device__ __forceinline__ void put_sums(float* o, int tid, int tpr, int D, const float2 (&f)[N]) {
+#pragma unroll
+  for (int e = 0; e < 2 * N; ++e) {
+    const int c = (e / VEC * tpr + tid) * VEC + e % VEC;
+    if (c < D) o[c] = e & 1 ? f[e >> 1].y : f[e >> 1].x;
+  }
+}
+
+// A run of rows per block, a row at a time with the next one's loads in flight; a thread
+// owns the same N pairs of columns in every row and keeps their sums in registers.
+// BIAS: S0 and T0 are wanted too.
 template <typename T, int VEC, int N, bool BIAS>
 __global__ void __launch_bounds__(512) backward_kernel(Params p) {
   __shared__ float part[2][MAX_WARPS * 2];
   RowSum<false, 2> sum{part};
   const int D = p.dim, tid = threadIdx.x, tpr = blockDim.x;
   const float inv_d = 1.f / D;
-  const int64_t group = blockIdx.x / p.segs, seg = blockIdx.x % p.segs;
-  const int64_t r0 = group * p.per + p.per * seg / p.segs, r1 = group * p.per + p.per * (seg + 1) / p.segs;
+  const int64_t r0 = p.rows * blockIdx.x / p.blocks, r1 = p.rows * (blockIdx.x + 1) / p.blocks;
+  float* const outS = p.part;
+  float* const outT = p.part + 2 * (p.blocks + p.groups) * D;
   float2 gw[N], gb[N], wp[N];  // gate w_post, gate b_post, w_pre
   float2 S1[N], T1[N], S0[N], T0[N];
-  load_vec<T, VEC, N>(p.w_post, p.vdt, 0, tid, tpr, D, gw);
   load_vec<T, VEC, N>(p.w_pre, p.vdt, 0, tid, tpr, D, wp);
 #pragma unroll
   for (int k = 0; k < N; ++k) S1[k] = T1[k] = S0[k] = T0[k] = gb[k] = two(0.f);
-  if (BIAS && p.b_post) load_vec<T, VEC, N>(p.b_post, p.vdt, 0, tid, tpr, D, gb);
-  if (p.gate) {
-    float2 g[N];
-    load_vec<T, VEC, N>(p.gate, p.vdt, group * D, tid, tpr, D, g);
+  int64_t group = r0 / p.per;
+  auto enter = [&]() {
+    load_vec<T, VEC, N>(p.w_post, p.vdt, 0, tid, tpr, D, gw);
+    if (BIAS && p.b_post) load_vec<T, VEC, N>(p.b_post, p.vdt, 0, tid, tpr, D, gb);
+    if (p.gate) {
+      float2 g[N];
+      load_vec<T, VEC, N>(p.gate, p.vdt, group * D, tid, tpr, D, g);
 #pragma unroll
-    for (int k = 0; k < N; ++k) gw[k] = __fmul2_rn(gw[k], g[k]), gb[k] = __fmul2_rn(gb[k], g[k]);
-  }
+      for (int k = 0; k < N; ++k) gw[k] = __fmul2_rn(gw[k], g[k]), gb[k] = __fmul2_rn(gb[k], g[k]);
+    }
+  };
+  auto leave = [&]() {
+    float* o = outS + (blockIdx.x + group) * D;
+    put_sums<VEC, N>(o, tid, tpr, D, S1);
+    if (BIAS) put_sums<VEC, N>(o + (p.blocks + p.groups) * D, tid, tpr, D, S0);
+  };
+  enter();
+  int64_t until = (group + 1) * p.per;  // the group's last row and one
   Raw<T, VEC, N> rx, rhh, ry, rd;
   float st[4];
   auto fetch = [&](int64_t r) {
@@ -300,6 +323,14 @@ __global__ void __launch_bounds__(512) backward_kernel(Params p) {
   };
   fetch(r0);
   for (int64_t r = r0; r < r1; ++r) {
+    if (r == until) {
+      leave();
+      ++group;
+      until += p.per;
+#pragma unroll
+      for (int k = 0; k < N; ++k) S1[k] = S0[k] = two(0.f);
+      enter();
+    }
     const float mh = st[0], rh = st[1], mz = st[2], rz = st[3];
     float2 hh[N], zh[N], dy[N], d[N];
     rx.get(zh);
@@ -348,46 +379,48 @@ __global__ void __launch_bounds__(512) backward_kernel(Params p) {
     store<T, VEC, N>(static_cast<T*>(p.dx) + r * D, tid, tpr, D, d);
     store<T, VEC, N>(static_cast<T*>(p.dh) + r * D, tid, tpr, D, hh);
   }
-  const int64_t n = p.units * D;
-  float* o = p.part + (int64_t)blockIdx.x * D;
-#pragma unroll
-  for (int e = 0; e < 2 * N; ++e) {
-    const int c = (e / VEC * tpr + tid) * VEC + e % VEC, k = e >> 1;
-    if (c >= D) continue;
-    o[c] = e & 1 ? S1[k].y : S1[k].x;
-    o[n + c] = e & 1 ? T1[k].y : T1[k].x;
-    if (BIAS) o[2 * n + c] = e & 1 ? S0[k].y : S0[k].x, o[3 * n + c] = e & 1 ? T0[k].y : T0[k].x;
-  }
+  leave();
+  put_sums<VEC, N>(outT + (int64_t)blockIdx.x * D, tid, tpr, D, T1);
+  if (BIAS) put_sums<VEC, N>(outT + (p.blocks + blockIdx.x) * D, tid, tpr, D, T0);
 }
 
-// The vectors' gradients from the units' sums, in two steps.  First, 32 columns per block:
-// part blockIdx.y of the groups (of the units, where there is one group), its 32 warps in
+// The vectors' gradients from the blocks' sums, in two steps.  First, 32 columns per block
+// and part blockIdx.y of the groups and of the backward pass's blocks, its 32 warps in
 // turn, added in order; the gates' gradients are complete here.
 template <bool BIAS>
 __global__ void __launch_bounds__(1024) gather_kernel(Params p, float* out) {
   __shared__ float acc[4][32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
-  const int64_t n = p.units * p.dim;
-  const bool many = p.groups > 1;
-  const int64_t runs = many ? p.groups : p.segs;
-  const int segs = many ? p.segs : 1;
+  const float* S = p.part + c;
+  const int64_t nS = (p.blocks + p.groups) * p.dim, nT = p.blocks * p.dim;
+  const float* R = S + 2 * nS;
+  const int64_t first = (int64_t)blockIdx.y * 32 + warp, step = gridDim.y * 32;
   float w = 0.f, b = 0.f, t1 = 0.f, t0 = 0.f;
   if (c < p.dim) {
-    for (int64_t g = (int64_t)blockIdx.y * 32 + warp; g < runs; g += gridDim.y * 32) {
-      float s1 = 0.f, s0 = 0.f;
-      for (int s = 0; s < segs; ++s) {
-        const float* q = p.part + (g * segs + s) * p.dim + c;
-        s1 += q[0];
-        t1 += q[n];
-        if (BIAS) s0 += q[2 * n], t0 += q[3 * n];
-      }
-      const float gt = many ? vec1(p.gate, p.vdt, g * p.dim + c, 1.f) : 1.f;
-      w += gt * s1;
-      b += gt * s0;
-      if (many)
+    if (p.groups > 1) {
+      for (int64_t g = first; g < p.groups; g += step) {
+        float s1 = 0.f, s0 = 0.f;
+        const int64_t k1 = p.blocks ? block_of(p, (g + 1) * p.per - 1) : -1;
+        for (int64_t k = p.blocks ? block_of(p, g * p.per) : 0; k <= k1; ++k) {
+          s1 += S[(k + g) * p.dim];
+          if (BIAS) s0 += S[nS + (k + g) * p.dim];
+        }
+        const float gt = vec1(p.gate, p.vdt, g * p.dim + c, 1.f);
+        w += gt * s1;
+        b += gt * s0;
         put1(p.dgate, p.vdt, g * p.dim + c,
              vec1(p.w_post, p.vdt, c, 1.f) * s1 + vec1(p.b_post, p.vdt, c, 0.f) * s0);
+      }
+    } else {
+      for (int64_t k = first; k < p.blocks; k += step) {
+        w += S[k * p.dim];
+        if (BIAS) b += S[nS + k * p.dim];
+      }
+    }
+    for (int64_t k = first; k < p.blocks; k += step) {
+      t1 += R[k * p.dim];
+      if (BIAS) t0 += R[nT + k * p.dim];
     }
   }
   acc[0][warp][lane] = w;
@@ -420,20 +453,18 @@ __global__ void __launch_bounds__(128) finish_kernel(Params p, const float* in, 
   put1(p.db_pre, p.vdt, c, s[3]);
 }
 
-constexpr int MAX_PARTS = 16;
-static int parts_of(int64_t groups, int segs) {
-  const int64_t runs = groups > 1 ? groups : segs;
-  int64_t n = (runs + 31) / 32;
-  return n < 1 ? 1 : n > MAX_PARTS ? MAX_PARTS : (int)n;
+// Blocks of the backward pass: what the SMs hold at 128 registers a thread, and at least
+// four rows each.
+static int64_t blocks_of(int64_t rows, int dim) {
+  const int pairs = dim <= 4096 ? 4 : dim <= 8192 ? 8 : 16;
+  const int tpr = (dim + 2 * pairs * 32 - 1) / (2 * pairs * 32) * 32;
+  const int64_t most = (int64_t)device_sm_count() * (512 / tpr > 8 ? 8 : 512 / tpr), n = (rows + 3) / 4;
+  return n < most ? n : most;
 }
-
-// Units per group: about `target` units in all, none without a row.
-static int segments(int64_t rows, int64_t groups) {
-  if (groups <= 0 || rows <= 0) return 1;
-  const int64_t per = rows / groups;
-  int64_t s = (int64_t)device_sm_count() * 5 / groups;
-  if (s > per) s = per;
-  return s < 1 ? 1 : (int)s;
+constexpr int MAX_PARTS = 16;
+static int parts_of(int64_t groups, int64_t blocks) {
+  const int64_t n = ((groups > blocks ? groups : blocks) + 31) / 32;
+  return n < 1 ? 1 : n > MAX_PARTS ? MAX_PARTS : (int)n;
 }
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -461,7 +492,7 @@ static void run_forward(const Params& p, cudaStream_t s) {
 template <typename T, int VEC, int N, bool BIAS>
 static void backward(const Params& p, cudaStream_t s) {
   const int tpr = (p.dim + 2 * N * 32 - 1) / (2 * N * 32) * 32;
-  backward_kernel<T, VEC, N, BIAS><<<(unsigned)p.units, tpr, 0, s>>>(p);
+  backward_kernel<T, VEC, N, BIAS><<<(unsigned)p.blocks, tpr, 0, s>>>(p);
 }
 
 template <typename T, int VEC, bool BIAS>
@@ -490,8 +521,8 @@ static void run(const Params& p, bool bwd, cudaStream_t s) {
     else if (bias) run_backward<T, 1, true>(p, s);
     else run_backward<T, 1, false>(p, s);
   }
-  const int parts = parts_of(p.groups, p.segs);
-  float* sums = p.part + 4 * p.units * p.dim;
+  const int parts = parts_of(p.groups, p.blocks);
+  float* sums = p.part + (4 * p.blocks + 2 * p.groups) * p.dim;
   const dim3 grid((unsigned)((p.dim + 31) / 32), (unsigned)parts);
   if (bias) gather_kernel<true><<<grid, 1024, 0, s>>>(p, sums);
   else gather_kernel<false><<<grid, 1024, 0, s>>>(p, sums);
@@ -542,8 +573,8 @@ int fms_norm_residual_fwd(int dtype, int vdtype, int kind, const void* x, const 
 
 size_t fms_norm_residual_bwd_workspace_size(int64_t rows, int64_t groups, int dim) {
   if (rows < 0 || groups < 0 || dim <= 0) return 0;
-  const int segs = rows > 0 ? norm::segments(rows, groups) : 0;
-  return ((size_t)groups * segs + norm::parts_of(groups, segs)) * 4 * dim * sizeof(float);
+  const int64_t blocks = norm::blocks_of(rows, dim);
+  return (size_t)(4 * blocks + 2 * groups + 4 * norm::parts_of(groups, blocks)) * dim * sizeof(float);
 }
 
 int fms_norm_residual_bwd(int dtype, int vdtype, int kind, const void* x, const void* h, const void* w_post,
@@ -564,8 +595,7 @@ int fms_norm_residual_bwd(int dtype, int vdtype, int kind, const void* x, const 
   p.stats = const_cast<float*>(stats); p.part = (float*)workspace;
   p.rows = rows; p.dim = dim; p.scale = scale;
   p.groups = groups;
-  p.segs = rows > 0 ? norm::segments(rows, groups) : 0;
-  p.units = groups * p.segs;
+  p.blocks = norm::blocks_of(rows, dim);
   p.per = groups > 0 ? rows / groups : 1;
   p.vdt = vdtype; p.layer = kind == FMS_NORM_LAYER;
   return norm::launch(dtype, p, true, (cudaStream_t)stream);
