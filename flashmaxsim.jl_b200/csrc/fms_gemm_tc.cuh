@@ -214,9 +214,9 @@ __device__ __forceinline__ Tile tile_at(const Work& w, int64_t t) {
 
 // ------------------------------------------------------------------ kernel
 
-// Epi::run(params, tile, row of the tile (rank * 128 + lane row), first column, TMEM
-// address of that column) handles the 32 lanes x BN/2 columns (BN/4 of each half for
-// OP_PAIR_B) of one epilogue warp.
+// Epi::run(params, tile, this lane's row of the product, half, TMEM address, ahead) handles
+// 32 lanes x every second 32 columns (`half` first) of an accumulator; Epi::fetch may load
+// what it needs for that into `ahead` while the products still run.
 template <int OP, int CG, int BN, bool A_MN, bool B_MN, bool I8, class Epi>
 __global__ void __launch_bounds__(NTHREADS, 1)
 kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensorMap tA1,
@@ -352,11 +352,14 @@ kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensor
     uint32_t bph = 0;
     for (int64_t t = first; t < tiles; t += stride) {
       const Tile T = tile_at(W, t);
+      const int64_t row = (int64_t)(T.m * CG + (int)rank) * MT + sub * 32 + lane;
+      typename Epi::template Ahead<BN> ahead;
+      Epi::template fetch<BN>(E, T, row, half, ahead);
       const bool ok = wait(&accf[buf], bph, &abort_s);
       if (!__all_sync(0xffffffffu, ok)) break;
       ptx::tc_fence_after();
       const uint32_t addr = tmem + buf * ACC + ((uint32_t)(sub * 32) << 16);
-      Epi::template run<BN>(E, T, (T.m * CG + (int)rank) * MT + sub * 32 + lane, half, addr);
+      Epi::template run<BN>(E, T, row, half, addr, ahead);
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -375,9 +378,9 @@ kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensor
 
 // ------------------------------------------------------------------ epilogue pieces
 
-// tcgen05.ld of 32 columns of this warp's lanes, complete on return.
-__device__ __forceinline__ void load32(uint32_t addr, uint32_t (&r)[32]) {
-  ptx::tmem_ld32(addr, r);
+// The loads so far are complete: ties the registers to the wait, so that no use of them
+// is scheduled before it.
+__device__ __forceinline__ void landed(uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.wait::ld.sync.aligned;"
       : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
@@ -387,6 +390,11 @@ __device__ __forceinline__ void load32(uint32_t addr, uint32_t (&r)[32]) {
         "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
       :
       : "memory");
+}
+// tcgen05.ld of 32 columns of this warp's lanes, complete on return.
+__device__ __forceinline__ void load32(uint32_t addr, uint32_t (&r)[32]) {
+  ptx::tmem_ld32(addr, r);
+  landed(r);
 }
 
 template <typename T>

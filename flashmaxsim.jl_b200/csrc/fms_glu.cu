@@ -31,32 +31,52 @@ struct HiddenEpi {
     int hidden, ldo;    // columns; elements between the rows of the outputs
     int wide, wide_dh;  // rows start on 32 bytes
   };
+  // The cotangents of a warp's columns, on their way while the products run.
   template <int BN>
-  static __device__ __forceinline__ void run(const Params& p, const Tile& t, int64_t row, int half, uint32_t addr) {
-#pragma unroll 1
-    for (int c = half; c < BN / 64; c += 2) {
+  struct Ahead {
+    uint32_t d[BWD ? (BN / 64 + 1) / 2 : 1][16];
+  };
+  template <int BN>
+  static __device__ __forceinline__ void fetch(const Params& p, const Tile& t, int64_t row, int half, Ahead<BN>& f) {
+    if constexpr (BWD) {
+#pragma unroll
+      for (int k = 0; k < (BN / 64 + 1) / 2; ++k) {
+        const int col = t.n * (BN / 2) + (2 * k + half) * 32;
+        const int n = row < p.rows && 2 * k + half < BN / 64 ? p.hidden - col : 0;
+        gemm::load_row32(p.dh + row * p.hidden + col, f.d[k], n, p.wide_dh);
+      }
+    }
+  }
+  template <int BN>
+  static __device__ __forceinline__ void run(const Params& p, const Tile& t, int64_t row, int half, uint32_t addr,
+                                             const Ahead<BN>& f) {
+#pragma unroll
+    for (int k = 0; k < (BN / 64 + 1) / 2; ++k) {
+      const int c = 2 * k + half;
+      if (c >= BN / 64) break;
       __syncwarp();
       uint32_t g[32], u[32];
-      gemm::load32(addr + c * 32, g);
-      gemm::load32(addr + BN / 2 + c * 32, u);
+      ptx::tmem_ld32(addr + c * 32, g);
+      gemm::load32(addr + BN / 2 + c * 32, u);  // waits for both
+      gemm::landed(g);
       const int col = t.n * (BN / 2) + c * 32;
       const int n = row < p.rows ? p.hidden - col : 0;
       if (n <= 0) continue;
-      uint32_t o[16], o1[16], d[16];
-      if (BWD) gemm::load_row32(p.dh + row * p.hidden + col, d, n, p.wide_dh);
+      uint32_t o[16], o1[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        float a0, a1, b0, b1;
-        const float g0 = __uint_as_float(g[2 * i]), g1 = __uint_as_float(g[2 * i + 1]);
-        const float u0 = __uint_as_float(u[2 * i]), u1 = __uint_as_float(u[2 * i + 1]);
-        act_eval<ACT, BWD>(g0, a0, b0);
-        act_eval<ACT, BWD>(g1, a1, b1);
+        float2 a, da;
+        const float2 gv = make_float2(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
+        const float2 uv = make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+        act_eval2<ACT, BWD>(gv, a, da);
         if (BWD) {
-          const float2 e = gemm::unpack2<T>(d[i]);
-          o[i] = gemm::pack2<T>(e.x * u0 * b0, e.y * u1 * b1);
-          o1[i] = gemm::pack2<T>(e.x * a0, e.y * a1);
+          const float2 e = gemm::unpack2<T>(f.d[k][i]);
+          const float2 x = __fmul2_rn(__fmul2_rn(e, uv), da), y = __fmul2_rn(e, a);
+          o[i] = gemm::pack2<T>(x.x, x.y);
+          o1[i] = gemm::pack2<T>(y.x, y.y);
         } else {
-          o[i] = gemm::pack2<T>(a0 * u0, a1 * u1);
+          const float2 x = __fmul2_rn(a, uv);
+          o[i] = gemm::pack2<T>(x.x, x.y);
         }
       }
       gemm::store_row32(p.o0 + row * p.ldo + col, o, n, p.wide);
@@ -78,7 +98,12 @@ struct StoreEpi {
     int wide;
   };
   template <int BN>
-  static __device__ __forceinline__ void run(const Params& p, const Tile& t, int64_t row, int half, uint32_t addr) {
+  struct Ahead {};
+  template <int BN>
+  static __device__ __forceinline__ void fetch(const Params&, const Tile&, int64_t, int, Ahead<BN>&) {}
+  template <int BN>
+  static __device__ __forceinline__ void run(const Params& p, const Tile& t, int64_t row, int half, uint32_t addr,
+                                             const Ahead<BN>&) {
     T* out = p.o0;
     int64_t at = t.split * (STACK ? 2 : 1) * p.rows;
     if (STACK && row >= p.pad) {
@@ -118,11 +143,27 @@ struct StoreEpi {
 // Sum of the parts of a split product, in order.
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int64_t each, T* o0, T* o1) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < 2 * each; i += (int64_t)gridDim.x * 256) {
+  const int64_t n = 2 * each;
+  if (each % 4 == 0 && ((reinterpret_cast<uintptr_t>(o0) | reinterpret_cast<uintptr_t>(o1)) & 7) == 0) {
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+      T* o = i < each ? o0 : o1;
+      if (!o) continue;
+      float4 s = *reinterpret_cast<const float4*>(part + i);
+#pragma unroll 4
+      for (int k = 1; k < splits; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(part + k * n + i);
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+      }
+      *reinterpret_cast<uint2*>(o + (i < each ? i : i - each)) =
+          make_uint2(gemm::pack2<T>(s.x, s.y), gemm::pack2<T>(s.z, s.w));
+    }
+    return;
+  }
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     T* o = i < each ? o0 : o1;
     if (!o) continue;
-    float s = 0.f;
-    for (int k = 0; k < splits; ++k) s += part[k * 2 * each + i];
+    float s = part[i];
+    for (int k = 1; k < splits; ++k) s += part[k * n + i];
     o[i < each ? i : i - each] = Tr<T>::from(s);
   }
 }

@@ -214,8 +214,12 @@ struct ScaleEpi {
     int wide;       // rows of y start on 32 bytes
   };
   template <int BN>
+  struct Ahead {};
+  template <int BN>
+  static __device__ __forceinline__ void fetch(const Params&, const gemm::Tile&, int64_t, int, Ahead<BN>&) {}
+  template <int BN>
   static __device__ __forceinline__ void run(const Params& p, const gemm::Tile& t, int64_t row, int half,
-                                             uint32_t addr) {
+                                             uint32_t addr, const Ahead<BN>&) {
     const float sx = row < p.rows ? __ldg(p.sx + row) : 0.f;
 #pragma unroll 1
     for (int c = half; c < BN / 32; c += 2) {
