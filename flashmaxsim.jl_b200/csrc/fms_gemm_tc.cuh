@@ -89,6 +89,12 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
   }
 }
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 template <int CG>
 __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   if (CG == 2)
@@ -319,30 +325,37 @@ kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensor
       ok = wait(&empty[s], ph ^ 1, &abort_s);
       if (++s == R::STAGES) s = 0, ph ^= 1;
     }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+  } else if (warp == 1 && rank == 0) {
     // ------------------------------------------------------------ MMA
+    // The whole warp runs the loop, so that descriptors stay in uniform registers; one
+    // elected lane issues.
+    const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint32_t ring_s = __shfl_sync(0xffffffffu, ptx::smem_u32(ring), 0);
     int s = 0, buf = 0;
     uint32_t ph = 0, bph = 0;
     bool ok = true;
     for (int64_t t = first; ok && t < tiles; t += stride) {
       const Tile T = tile_at(W, t);
-      if (!wait(&acce[buf], bph ^ 1, &abort_s)) break;
+      if (!__all_sync(0xffffffffu, wait(&acce[buf], bph ^ 1, &abort_s))) break;
       ptx::tc_fence_after();
-      const uint32_t d = tmem + buf * ACC;
+      const uint32_t d = base + buf * ACC;
       for (int kb = T.k0; kb < T.k1; ++kb) {
-        if (!wait(&full[s], ph, &abort_s)) {
+        if (!__all_sync(0xffffffffu, wait(&full[s], ph, &abort_s))) {
           ok = false;
           break;
         }
-        ptx::tc_fence_after();
-        const uint32_t a = ptx::smem_u32(ring + s * R::STAGE), b = a + R::A_BYTES;
+        const uint32_t a = ring_s + s * R::STAGE, b = a + R::A_BYTES;
+        if (elect_one()) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          mma<CG, I8>(d, desc<A_MN>(a + j * KSTEP), desc<B_MN>(b + j * KSTEP_B), W.idesc, kb > T.k0 || j > 0);
-        commit<CG>(&empty[s]);
+          for (int j = 0; j < 4; ++j)
+            mma<CG, I8>(d, desc<A_MN>(a + j * KSTEP), desc<B_MN>(b + j * KSTEP_B), W.idesc, kb > T.k0 || j > 0);
+          commit<CG>(&empty[s]);
+        }
+        __syncwarp();
         if (++s == R::STAGES) s = 0, ph ^= 1;
       }
-      commit<CG>(&accf[buf]);
+      if (elect_one()) commit<CG>(&accf[buf]);
+      __syncwarp();
       if (++buf == 2) buf = 0, bph ^= 1;
     }
   } else if (warp >= 2) {
