@@ -96,17 +96,17 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 template <int CG>
-__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   if (CG == 2)
     asm volatile(
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%2, %3}], [%4];" ::"r"(ptx::smem_u32(dst)),
+        "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
         : "memory");
   else
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%2, %3}], [%4];" ::"r"(ptx::smem_u32(dst)),
+        "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
@@ -264,57 +264,47 @@ kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensor
   const int64_t tiles = (int64_t)W.mt * W.nt * W.splits;
   const int64_t first = blockIdx.x / CG, stride = gridDim.x / CG;
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     // ------------------------------------------------------------ loads
+    // Like the MMA warp: all lanes run the loop, an elected one issues.
+    const uint32_t ring_s = __shfl_sync(0xffffffffu, ptx::smem_u32(ring), 0);
+    const uint32_t full_s = __shfl_sync(0xffffffffu, CG == 2 ? cluster_addr(full, 0) : ptx::smem_u32(full), 0);
+    const int rk = __shfl_sync(0xffffffffu, (int)rank, 0);
     int s = 0;
     uint32_t ph = 0;
     bool ok = true;
     for (int64_t t = first; ok && t < tiles; t += stride) {
       const Tile T = tile_at(W, t);
+      const bool second = OP == OP_STACK_A && T.m >= W.mt0;
+      const int m0 = (((second ? T.m - W.mt0 : T.m)) * CG + rk) * MT;
+      const int n0 = OP == OP_PAIR_B ? T.n * (BN / 2) : T.n * BN + rk * (BN / CG);
       for (int kb = T.k0; kb < T.k1; ++kb) {
-        if (!wait(&empty[s], ph ^ 1, &abort_s)) {
+        if (!__all_sync(0xffffffffu, wait(&empty[s], ph ^ 1, &abort_s))) {
           ok = false;
           break;
         }
-        unsigned char* a = ring + s * R::STAGE;
-        unsigned char* b = a + R::A_BYTES;
-        if (rank == 0) ptx::mbar_expect_tx(&full[s], CG * R::STAGE);
-        const uint32_t bar = CG == 2 ? cluster_addr(&full[s], 0) : ptx::smem_u32(&full[s]);
-        const CUtensorMap* mA = &tA0;
-        int k = kb, m0 = T.m * CG;
-        if (OP == OP_SUM && kb >= W.kb0) {
-          mA = &tA1;
-          k -= W.kb0;
-        }
-        if (OP == OP_STACK_A && T.m >= W.mt0) {
-          mA = &tA1;
-          m0 = (T.m - W.mt0) * CG;
-        }
-        m0 = (m0 + (int)rank) * MT;
-        if (A_MN) {
+        const uint32_t a = ring_s + s * R::STAGE, b = a + R::A_BYTES, bar = full_s + s * 8;
+        const bool next = OP == OP_SUM && kb >= W.kb0;
+        const int k = next ? kb - W.kb0 : kb;
+        if (elect_one()) {
+          if (rk == 0) ptx::mbar_expect_tx(&full[s], CG * R::STAGE);
+          const CUtensorMap* mA = second || next ? &tA1 : &tA0;
+          const CUtensorMap* mB = next || (OP == OP_PAIR_B && CG == 2 && rk == 1) ? &tB1 : &tB0;
+          if (A_MN) {
 #pragma unroll
-          for (int c = 0; c < MT / 64; ++c) tma_load<CG>(a + c * 8192, mA, m0 + c * 64, k * 64, bar);
-        } else {
-          tma_load<CG>(a, mA, k * KEL, m0, bar);
-        }
-        if (OP == OP_PAIR_B) {
-          const int n0 = T.n * (BN / 2);
-          if (CG == 2) {
-            tma_load<CG>(b, rank == 0 ? &tB0 : &tB1, k * KEL, n0, bar);
+            for (int c = 0; c < MT / 64; ++c) tma_load<CG>(a + c * 8192, mA, m0 + c * 64, k * 64, bar);
           } else {
-            tma_load<CG>(b, &tB0, k * KEL, n0, bar);
-            tma_load<CG>(b + R::B_BYTES / 2, &tB1, k * KEL, n0, bar);
+            tma_load<CG>(a, mA, k * KEL, m0, bar);
           }
-        } else {
-          const CUtensorMap* mB = OP == OP_SUM && kb >= W.kb0 ? &tB1 : &tB0;
-          const int n0 = T.n * BN + (int)rank * (BN / CG);
           if (B_MN) {
 #pragma unroll
             for (int c = 0; c < BN / CG / 64; ++c) tma_load<CG>(b + c * 8192, mB, n0 + c * 64, k * 64, bar);
           } else {
             tma_load<CG>(b, mB, k * KEL, n0, bar);
+            if (OP == OP_PAIR_B && CG == 1) tma_load<CG>(b + R::B_BYTES / 2, &tB1, k * KEL, n0, bar);
           }
         }
+        __syncwarp();
         if (++s == R::STAGES) s = 0, ph ^= 1;
       }
     }
@@ -322,7 +312,7 @@ kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensor
     // In the leader every stage's barrier completes when both CTAs' copies have landed;
     // the other CTA's stages are released by the leader's commits.
     for (int i = 0; ok && i < R::STAGES; ++i) {
-      ok = wait(&empty[s], ph ^ 1, &abort_s);
+      ok = __all_sync(0xffffffffu, wait(&empty[s], ph ^ 1, &abort_s));
       if (++s == R::STAGES) s = 0, ph ^= 1;
     }
   } else if (warp == 1 && rank == 0) {
