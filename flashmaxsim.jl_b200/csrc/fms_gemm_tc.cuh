@@ -31,7 +31,8 @@ constexpr int MT = 128;         // accumulator rows of a CTA
 constexpr int NEPI = 8;         // epilogue warps
 constexpr int NTHREADS = (2 + NEPI) * 32;
 constexpr int ROWB = 128;       // bytes of a stage row (one swizzle atom wide)
-constexpr int SMEM_BYTES = 200 * 1024;  // stages; the rest of 227 KB is barriers and slack
+constexpr int SMEM_BYTES = 192 * 1024;  // ring stages
+constexpr int OUT_BYTES = 4096;         // per epilogue warp: 32 rows x 64 16-bit columns on their way out
 
 template <int BN, int CG>
 struct Ring {
@@ -220,14 +221,15 @@ __device__ __forceinline__ Tile tile_at(const Work& w, int64_t t) {
 
 // ------------------------------------------------------------------ kernel
 
-// Epi::run(params, tile, this lane's row of the product, half, TMEM address, ahead) handles
-// 32 lanes x every second 32 columns (`half` first) of an accumulator; Epi::fetch may load
-// what it needs for that into `ahead` while the products still run.
+// Epi::run(params, tile, this lane's row of the product, half, TMEM address, ahead, out)
+// handles 32 lanes x half of the columns of an accumulator (of either half of it for
+// OP_PAIR_B); Epi::fetch may load what it needs for that into `ahead` while the products
+// still run; `out` is the warp's OUT_BYTES of shared memory.
 template <int OP, int CG, int BN, bool A_MN, bool B_MN, bool I8, class Epi>
 __global__ void __launch_bounds__(NTHREADS, 1)
 kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensorMap tA1,
        const __grid_constant__ CUtensorMap tB0, const __grid_constant__ CUtensorMap tB1, const Work W,
-       const typename Epi::Params E) {
+       const __grid_constant__ typename Epi::Params E) {
   using R = Ring<BN, CG>;
   constexpr int KEL = I8 ? 128 : 64;                // sum elements of a stage
   constexpr int KSTEP = A_MN ? 2048 : 32;           // descriptor bytes of one MMA's sum (16 or 32 elements)
@@ -351,6 +353,7 @@ kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensor
   } else if (warp >= 2) {
     // ------------------------------------------------------------ epilogue
     const int sub = warp & 3, half = (warp - 2) >> 2;
+    unsigned char* const out = ring + R::STAGES * R::STAGE + (warp - 2) * OUT_BYTES;
     int buf = 0;
     uint32_t bph = 0;
     for (int64_t t = first; t < tiles; t += stride) {
@@ -362,7 +365,7 @@ kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensor
       if (!__all_sync(0xffffffffu, ok)) break;
       ptx::tc_fence_after();
       const uint32_t addr = tmem + buf * ACC + ((uint32_t)(sub * 32) << 16);
-      Epi::template run<BN>(E, T, row, half, addr, ahead);
+      Epi::template run<BN>(E, T, row, half, addr, ahead, out);
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -371,6 +374,7 @@ kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensor
       }
       if (++buf == 2) buf = 0, bph ^= 1;
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // stores out of `out`
   }
   __syncwarp();
   __syncthreads();
@@ -463,6 +467,35 @@ __device__ __forceinline__ void load_row32(const T* p, uint32_t (&v)[16], int n,
   }
 }
 
+// The same 32 values of column group 0 or 1 of 64 into the warp's `out`, in the 128-byte
+// swizzle that the store's map names.  A store of whole 128-byte lines by the copy engine:
+// stores by lane, each to a row of its own, held up the epilogue (dg and du of 46080 x 2048:
+// 281 us against 2xx).
+__device__ __forceinline__ void put32(unsigned char* out, int lane, int group, const uint32_t (&v)[16]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    *reinterpret_cast<uint4*>(out + lane * 128 + (((group * 4 + q) ^ (lane & 7)) << 4)) =
+        make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+}
+// `out` is free again: its last store has been read out of it (all lanes).
+__device__ __forceinline__ void out_free(int lane) {
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  __syncwarp();
+}
+// 64 columns x 32 rows of `out` to (col, row) (all lanes; rows and columns past the map's
+// end are left out).
+__device__ __forceinline__ void out_store(const unsigned char* out, const CUtensorMap* map, int col, int row, int lane) {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  if (lane == 0) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(col), "r"(row), "r"(ptx::smem_u32(out))
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+}
+
 // ------------------------------------------------------------------ host side
 
 inline uint32_t idesc_f16(int dtype, int M, int N, bool a_mn, bool b_mn) {
@@ -498,7 +531,7 @@ template <int OP, int CG, int BN, bool A_MN, bool B_MN, bool I8, class Epi>
 cudaError_t launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& b0, const CUtensorMap& b1,
                    const Work& w, const typename Epi::Params& e, int sms, cudaStream_t s) {
   auto k = kernel<OP, CG, BN, A_MN, B_MN, I8, Epi>;
-  constexpr int smem = Ring<BN, CG>::STAGES * Ring<BN, CG>::STAGE + 1024;
+  constexpr int smem = Ring<BN, CG>::STAGES * Ring<BN, CG>::STAGE + NEPI * OUT_BYTES + 1024;
   cudaError_t err = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (err != cudaSuccess) return err;
   const int64_t tiles = (int64_t)w.mt * w.nt * w.splits;

@@ -24,45 +24,49 @@ using gemm::Tile;
 // h = a(g) u, or with BWD dg = dh u a'(g) and du = dh a(g).
 template <typename T, int ACT, bool BWD>
 struct HiddenEpi {
-  struct Params {
+  struct alignas(64) Params {
+    CUtensorMap m0, m1;  // o0 and o1, where `mapped`
     const T* dh;
-    T *o0, *o1;         // h, or dg and du
+    T *o0, *o1;          // h, or dg and du
     int64_t rows;
-    int hidden, ldo;    // columns; elements between the rows of the outputs
-    int wide, wide_dh;  // rows start on 32 bytes
+    int hidden, ldo;     // columns; elements between the rows of the outputs
+    int wide, wide_dh;   // rows start on 32 bytes
+    int mapped;          // rows start on 16 bytes, as the copy engine's stores ask
   };
+  static __host__ __device__ constexpr int GROUPS(int BN) { return BN >= 128 ? BN / 128 : 1; }  // of 32 columns of a warp
   // The cotangents of a warp's columns, on their way while the products run.
   template <int BN>
   struct Ahead {
-    uint32_t d[BWD ? (BN / 64 + 1) / 2 : 1][16];
+    uint32_t d[BWD ? GROUPS(BN) : 1][16];
   };
   template <int BN>
   static __device__ __forceinline__ void fetch(const Params& p, const Tile& t, int64_t row, int half, Ahead<BN>& f) {
     if constexpr (BWD) {
 #pragma unroll
-      for (int k = 0; k < (BN / 64 + 1) / 2; ++k) {
-        const int col = t.n * (BN / 2) + (2 * k + half) * 32;
-        const int n = row < p.rows && 2 * k + half < BN / 64 ? p.hidden - col : 0;
+      for (int k = 0; k < GROUPS(BN); ++k) {
+        const int c = half * GROUPS(BN) + k, col = t.n * (BN / 2) + c * 32;
+        const int n = row < p.rows && c < BN / 64 ? p.hidden - col : 0;
         gemm::load_row32(p.dh + row * p.hidden + col, f.d[k], n, p.wide_dh);
       }
     }
   }
   template <int BN>
   static __device__ __forceinline__ void run(const Params& p, const Tile& t, int64_t row, int half, uint32_t addr,
-                                             const Ahead<BN>& f) {
+                                             const Ahead<BN>& f, unsigned char* out) {
+    const int lane = threadIdx.x & 31;
+    const bool mapped = GROUPS(BN) == 2 && p.mapped;  // 64 columns: whole lines
+    const int col0 = t.n * (BN / 2) + half * GROUPS(BN) * 32;
+    uint32_t keep[GROUPS(BN)][16];
 #pragma unroll
-    for (int k = 0; k < (BN / 64 + 1) / 2; ++k) {
-      const int c = 2 * k + half;
+    for (int k = 0; k < GROUPS(BN); ++k) {
+      const int c = half * GROUPS(BN) + k;
       if (c >= BN / 64) break;
       __syncwarp();
       uint32_t g[32], u[32];
       ptx::tmem_ld32(addr + c * 32, g);
       gemm::load32(addr + BN / 2 + c * 32, u);  // waits for both
       gemm::landed(g);
-      const int col = t.n * (BN / 2) + c * 32;
-      const int n = row < p.rows ? p.hidden - col : 0;
-      if (n <= 0) continue;
-      uint32_t o[16], o1[16];
+      uint32_t o[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float2 a, da;
@@ -73,14 +77,31 @@ struct HiddenEpi {
           const float2 e = gemm::unpack2<T>(f.d[k][i]);
           const float2 x = __fmul2_rn(__fmul2_rn(e, uv), da), y = __fmul2_rn(e, a);
           o[i] = gemm::pack2<T>(x.x, x.y);
-          o1[i] = gemm::pack2<T>(y.x, y.y);
+          keep[k][i] = gemm::pack2<T>(y.x, y.y);
         } else {
           const float2 x = __fmul2_rn(a, uv);
           o[i] = gemm::pack2<T>(x.x, x.y);
         }
       }
-      gemm::store_row32(p.o0 + row * p.ldo + col, o, n, p.wide);
-      if (BWD) gemm::store_row32(p.o1 + row * p.ldo + col, o1, n, p.wide);
+      if (mapped) {
+        if (k == 0) gemm::out_free(lane);
+        gemm::put32(out, lane, k, o);
+      } else {
+        const int col = col0 + k * 32, n = row < p.rows ? p.hidden - col : 0;
+        if (n > 0) {
+          gemm::store_row32(p.o0 + row * p.ldo + col, o, n, p.wide);
+          if (BWD) gemm::store_row32(p.o1 + row * p.ldo + col, keep[k], n, p.wide);
+        }
+      }
+    }
+    const int64_t row0 = row - lane;
+    if (!mapped || col0 >= p.hidden || row0 >= p.rows) return;
+    gemm::out_store(out, &p.m0, col0, (int)row0, lane);
+    if (BWD) {
+      gemm::out_free(lane);
+#pragma unroll
+      for (int k = 0; k < GROUPS(BN); ++k) gemm::put32(out, lane, k, keep[k]);
+      gemm::out_store(out, &p.m1, col0, (int)row0, lane);
     }
   }
 };
@@ -90,12 +111,13 @@ struct HiddenEpi {
 // outputs, `pad` rows of tiles each.
 template <typename T, bool STACK>
 struct StoreEpi {
-  struct Params {
+  struct alignas(64) Params {
+    CUtensorMap m0, m1;  // o0 and o1, where `mapped`
     T *o0, *o1;
     float* part;
     int64_t rows, pad;
     int cols;
-    int wide;
+    int wide, mapped;
   };
   template <int BN>
   struct Ahead {};
@@ -103,23 +125,27 @@ struct StoreEpi {
   static __device__ __forceinline__ void fetch(const Params&, const Tile&, int64_t, int, Ahead<BN>&) {}
   template <int BN>
   static __device__ __forceinline__ void run(const Params& p, const Tile& t, int64_t row, int half, uint32_t addr,
-                                             const Ahead<BN>&) {
+                                             const Ahead<BN>&, unsigned char* stage) {
+    static_assert(BN >= 128, "64 columns to a warp");
+    const int lane = threadIdx.x & 31;
     T* out = p.o0;
+    const CUtensorMap* map = &p.m0;
     int64_t at = t.split * (STACK ? 2 : 1) * p.rows;
     if (STACK && row >= p.pad) {
       row -= p.pad;
       out = p.o1;
+      map = &p.m1;
       at += p.rows;
     }
 #pragma unroll 1
-    for (int c = half; c < BN / 32; c += 2) {
+    for (int c = half * (BN / 64); c < (half + 1) * (BN / 64); ++c) {
       __syncwarp();
       uint32_t v[32];
       gemm::load32(addr + c * 32, v);
       const int col = t.n * BN + c * 32;
       const int n = row < p.rows ? p.cols - col : 0;
-      if (n <= 0) continue;
       if (p.part) {
+        if (n <= 0) continue;
         float* q = p.part + (at + row) * p.cols + col;
         if (n >= 32 && p.wide) {
 #pragma unroll
@@ -134,7 +160,14 @@ struct StoreEpi {
         uint32_t o[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i] = gemm::pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-        gemm::store_row32(out + row * p.cols + col, o, n, p.wide);
+        if (p.mapped) {
+          if ((c & 1) == 0) gemm::out_free(lane);
+          gemm::put32(stage, lane, c & 1, o);
+          if ((c & 1) && col - 32 < p.cols && row - lane < p.rows)
+            gemm::out_store(stage, map, col - 32, (int)(row - lane), lane);
+        } else if (n > 0) {
+          gemm::store_row32(out + row * p.cols + col, o, n, p.wide);
+        }
       }
     }
   }
@@ -264,6 +297,9 @@ static cudaError_t hidden_pass(int dtype, const void* x, const void* wg, const v
   e.ldo = ldo;
   e.wide = ldo % 16 == 0 && aligned(o0, 32) && (!BWD || aligned(o1, 32));
   e.wide_dh = p.hidden % 16 == 0 && aligned(p.dh, 32);
+  e.mapped = BN == 256 && ldo % 8 == 0 && aligned(o0, 16) && (!BWD || aligned(o1, 16)) &&
+             gemm::make_map(&e.m0, dtype, o0, p.hidden, p.rows, (int64_t)ldo * 2, 32) &&
+             (!BWD || gemm::make_map(&e.m1, dtype, o1, p.hidden, p.rows, (int64_t)ldo * 2, 32));
   return gemm::launch<gemm::OP_PAIR_B, CG, BN, false, false, false, HiddenEpi<T, ACT, BWD>>(a, a, b0, b1, w, e,
                                                                                             device_sm_count(), s);
 }
@@ -297,6 +333,7 @@ static cudaError_t input_gradient(int dtype, const T* dg, const T* du, const voi
   e.rows = p.rows;
   e.cols = p.dim;
   e.wide = p.dim % 16 == 0 && aligned(p.dx, 32);
+  e.mapped = p.dim % 8 == 0 && aligned(p.dx, 16) && gemm::make_map(&e.m0, dtype, p.dx, p.dim, p.rows, (int64_t)p.dim * 2, 32);
   return gemm::launch<gemm::OP_SUM, 2, 256, false, true, false, StoreEpi<T, false>>(a0, a1, b0, b1, w, e,
                                                                                     device_sm_count(), s);
 }
@@ -325,6 +362,9 @@ static cudaError_t weight_gradients(int dtype, const T* dg, const T* du, const v
   e.pad = (int64_t)w.mt0 * 256;
   e.cols = p.dim;
   e.wide = e.part ? p.dim % 4 == 0 : p.dim % 16 == 0 && aligned(p.dwg, 32) && aligned(p.dwu, 32);
+  e.mapped = !e.part && p.dim % 8 == 0 && p.dwg && p.dwu && aligned(p.dwg, 16) && aligned(p.dwu, 16) &&
+             gemm::make_map(&e.m0, dtype, p.dwg, p.dim, p.hidden, (int64_t)p.dim * 2, 32) &&
+             gemm::make_map(&e.m1, dtype, p.dwu, p.dim, p.hidden, (int64_t)p.dim * 2, 32);
   const cudaError_t err = gemm::launch<gemm::OP_STACK_A, 2, 256, true, true, false, StoreEpi<T, true>>(
       a0, a1, b, b, w, e, device_sm_count(), s);
   if (err != cudaSuccess || splits == 1) return err;

@@ -13,6 +13,8 @@
 #include "fms_gemm_tc.cuh"
 #include "fms_internal.h"
 
+#include <type_traits>
+
 namespace fms {
 namespace lin8 {
 
@@ -205,13 +207,15 @@ __global__ void __launch_bounds__(256) few_kernel(const X* x, const float* x_sca
 
 template <typename Y>
 struct ScaleEpi {
-  struct Params {
+  struct alignas(64) Params {
+    CUtensorMap map;  // y, where `mapped`
     const float *sx, *sw;
     const Y* bias;
     Y* y;
     int64_t rows;
     int cols;
-    int wide;       // rows of y start on 32 bytes
+    int wide;         // rows of y start on 32 bytes
+    int mapped;       // 16-bit rows that start on 16 bytes, 64 columns to a warp
   };
   template <int BN>
   struct Ahead {};
@@ -219,20 +223,21 @@ struct ScaleEpi {
   static __device__ __forceinline__ void fetch(const Params&, const gemm::Tile&, int64_t, int, Ahead<BN>&) {}
   template <int BN>
   static __device__ __forceinline__ void run(const Params& p, const gemm::Tile& t, int64_t row, int half,
-                                             uint32_t addr, const Ahead<BN>&) {
+                                             uint32_t addr, const Ahead<BN>&, unsigned char* stage) {
+    const int lane = threadIdx.x & 31;
     const float sx = row < p.rows ? __ldg(p.sx + row) : 0.f;
 #pragma unroll 1
-    for (int c = half; c < BN / 32; c += 2) {
+    for (int c = half * (BN / 64); c < (half + 1) * (BN / 64); ++c) {
       __syncwarp();
       uint32_t v[32];
       gemm::load32(addr + c * 32, v);
       const int col = t.n * BN + c * 32;
       const int n = row < p.rows ? p.cols - col : 0;
-      if (n <= 0) continue;
       float f[32];
+      // columns past the end take the last one's scale; they are not stored
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        const int at = i < n ? col + i : col;
+        const int at = min(col + i, p.cols - 1);
         f[i] = (sx * __ldg(p.sw + at)) * (float)(int32_t)v[i];
         if (p.bias) f[i] += Tr<Y>::to(p.bias[at]);
       }
@@ -241,14 +246,21 @@ struct ScaleEpi {
         uint32_t o[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i] = gemm::pack2<Y>(f[2 * i], f[2 * i + 1]);
-        gemm::store_row32(out, o, n, p.wide);
-      } else {
+        if (BN >= 128 && p.mapped) {
+          if ((c & 1) == 0) gemm::out_free(lane);
+          gemm::put32(stage, lane, c & 1, o);
+          if ((c & 1) && col - 32 < p.cols && row - lane < p.rows)
+            gemm::out_store(stage, &p.map, col - 32, (int)(row - lane), lane);
+        } else if (n > 0) {
+          gemm::store_row32(out, o, n, p.wide);
+        }
+      } else if (n > 0) {
         uint32_t o[16];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {  // 16 floats are 32 half-words
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(f[16 * h + i]);
-          gemm::store_row32(reinterpret_cast<uint16_t*>(out + 16 * h), o, 2 * (n - 16 * h), p.wide);
+          if (n > 16 * h) gemm::store_row32(reinterpret_cast<uint16_t*>(out + 16 * h), o, 2 * (n - 16 * h), p.wide);
         }
       }
     }
@@ -356,6 +368,9 @@ static cudaError_t product(const int8_t* xc, const float* sx, const int8_t* wc, 
   e.rows = p.rows;
   e.cols = p.C;
   e.wide = (p.C * sizeof(Y)) % 32 == 0 && aligned(p.y, 32);
+  e.mapped = sizeof(Y) == 2 && BN >= 128 && p.C % 8 == 0 && aligned(p.y, 16) &&
+             gemm::make_map(&e.map, std::is_same<Y, __half>::value ? FMS_F16 : FMS_BF16, p.y, p.C, p.rows,
+                            (int64_t)p.C * 2, 32);
   return gemm::launch<gemm::OP_ONE, CG, BN, false, false, true, ScaleEpi<Y>>(a, a, b, b, w, e, device_sm_count(), s);
 }
 
