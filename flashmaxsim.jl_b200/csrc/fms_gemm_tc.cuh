@@ -58,8 +58,10 @@ __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(ptx::smem_u32(p)), "r"(rank));
   return a;
 }
+// Arrive on a barrier of the cluster.  Ordered after the warp's TMEM reads by the fence
+// before it; release at cluster scope would wait for the epilogue's stores as well.
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 __device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -221,10 +223,11 @@ __device__ __forceinline__ Tile tile_at(const Work& w, int64_t t) {
 
 // ------------------------------------------------------------------ kernel
 
-// Epi::run(params, tile, this lane's row of the product, half, TMEM address, ahead, out)
-// handles 32 lanes x half of the columns of an accumulator (of either half of it for
+// Epi::run(params, tile, this lane's row of the product, half, TMEM address, ahead, out,
+// release) handles 32 lanes x half of the columns of an accumulator (of either half of it for
 // OP_PAIR_B); Epi::fetch may load what it needs for that into `ahead` while the products
-// still run; `out` is the warp's OUT_BYTES of shared memory.
+// still run; `out` is the warp's OUT_BYTES of shared memory; it calls `release` once, when
+// it has read the accumulator.
 template <int OP, int CG, int BN, bool A_MN, bool B_MN, bool I8, class Epi>
 __global__ void __launch_bounds__(NTHREADS, 1)
 kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensorMap tA1,
@@ -365,13 +368,14 @@ kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensor
       if (!__all_sync(0xffffffffu, ok)) break;
       ptx::tc_fence_after();
       const uint32_t addr = tmem + buf * ACC + ((uint32_t)(sub * 32) << 16);
-      Epi::template run<BN>(E, T, row, half, addr, ahead, out);
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (CG == 2) arrive_cluster(cluster_addr(&acce[buf], 0));
-        else ptx::mbar_arrive(&acce[buf]);
-      }
+      Epi::template run<BN>(E, T, row, half, addr, ahead, out, [&]() {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (CG == 2) arrive_cluster(cluster_addr(&acce[buf], 0));
+          else ptx::mbar_arrive(&acce[buf]);
+        }
+      });
       if (++buf == 2) buf = 0, bph ^= 1;
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // stores out of `out`

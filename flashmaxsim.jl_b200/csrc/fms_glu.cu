@@ -50,9 +50,9 @@ struct HiddenEpi {
       }
     }
   }
-  template <int BN>
+  template <int BN, class Release>
   static __device__ __forceinline__ void run(const Params& p, const Tile& t, int64_t row, int half, uint32_t addr,
-                                             const Ahead<BN>& f, unsigned char* out) {
+                                             const Ahead<BN>& f, unsigned char* out, Release release) {
     const int lane = threadIdx.x & 31;
     const bool mapped = GROUPS(BN) == 2 && p.mapped;  // 64 columns: whole lines
     const int col0 = t.n * (BN / 2) + half * GROUPS(BN) * 32;
@@ -60,12 +60,16 @@ struct HiddenEpi {
 #pragma unroll
     for (int k = 0; k < GROUPS(BN); ++k) {
       const int c = half * GROUPS(BN) + k;
-      if (c >= BN / 64) break;
+      if (c >= BN / 64) {
+        release();
+        break;
+      }
       __syncwarp();
       uint32_t g[32], u[32];
       ptx::tmem_ld32(addr + c * 32, g);
       gemm::load32(addr + BN / 2 + c * 32, u);  // waits for both
       gemm::landed(g);
+      if (k == GROUPS(BN) - 1) release();
       uint32_t o[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -123,9 +127,9 @@ struct StoreEpi {
   struct Ahead {};
   template <int BN>
   static __device__ __forceinline__ void fetch(const Params&, const Tile&, int64_t, int, Ahead<BN>&) {}
-  template <int BN>
+  template <int BN, class Release>
   static __device__ __forceinline__ void run(const Params& p, const Tile& t, int64_t row, int half, uint32_t addr,
-                                             const Ahead<BN>&, unsigned char* stage) {
+                                             const Ahead<BN>&, unsigned char* stage, Release release) {
     static_assert(BN >= 128, "64 columns to a warp");
     const int lane = threadIdx.x & 31;
     T* out = p.o0;
@@ -142,6 +146,7 @@ struct StoreEpi {
       __syncwarp();
       uint32_t v[32];
       gemm::load32(addr + c * 32, v);
+      if (c + 1 == (half + 1) * (BN / 64)) release();
       const int col = t.n * BN + c * 32;
       const int n = row < p.rows ? p.cols - col : 0;
       if (p.part) {

@@ -221,9 +221,9 @@ struct ScaleEpi {
   struct Ahead {};
   template <int BN>
   static __device__ __forceinline__ void fetch(const Params&, const gemm::Tile&, int64_t, int, Ahead<BN>&) {}
-  template <int BN>
-  static __device__ __forceinline__ void run(const Params& p, const gemm::Tile& t, int64_t row, int half,
-                                             uint32_t addr, const Ahead<BN>&, unsigned char* stage) {
+  template <int BN, class Release>
+  static __device__ __forceinline__ void run(const Params& p, const gemm::Tile& t, int64_t row, int half, uint32_t addr,
+                                             const Ahead<BN>&, unsigned char* stage, Release release) {
     const int lane = threadIdx.x & 31;
     const float sx = row < p.rows ? __ldg(p.sx + row) : 0.f;
 #pragma unroll 1
@@ -231,6 +231,7 @@ struct ScaleEpi {
       __syncwarp();
       uint32_t v[32];
       gemm::load32(addr + c * 32, v);
+      if (c + 1 == (half + 1) * (BN / 64)) release();
       const int col = t.n * BN + c * 32;
       const int n = row < p.rows ? p.cols - col : 0;
       float f[32];
