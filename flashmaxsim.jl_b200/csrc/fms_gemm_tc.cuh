@@ -431,30 +431,11 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
   return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
 }
 
-// 32 consecutive 16-bit values of one row (two per register) to p; `n` of them exist.
-// wide: p and the rows' stride are multiples of 32 bytes, so that whole 32-byte
-// sectors go out (a 16-byte store leaves half of one to be merged).
+// 32 consecutive 16-bit values of one row (two per register); `n` of them exist, rows
+// start on 32 bytes.
 template <typename T>
-__device__ __forceinline__ void store_row32(T* p, const uint32_t (&v)[16], int n, bool wide) {
-  if (n >= 32 && wide) {
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
-      asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p + 16 * q), "r"(v[8 * q]),
-                   "r"(v[8 * q + 1]), "r"(v[8 * q + 2]), "r"(v[8 * q + 3]), "r"(v[8 * q + 4]), "r"(v[8 * q + 5]),
-                   "r"(v[8 * q + 6]), "r"(v[8 * q + 7])
-                   : "memory");
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < n) {
-        const uint16_t h = (uint16_t)(i & 1 ? v[i >> 1] >> 16 : v[i >> 1]);
-        reinterpret_cast<uint16_t*>(p)[i] = h;
-      }
-  }
-}
-template <typename T>
-__device__ __forceinline__ void load_row32(const T* p, uint32_t (&v)[16], int n, bool wide) {
-  if (n >= 32 && wide) {
+__device__ __forceinline__ void load_row32(const T* p, uint32_t (&v)[16], int n) {
+  if (n >= 32) {
 #pragma unroll
     for (int q = 0; q < 2; ++q)
       asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -471,14 +452,19 @@ __device__ __forceinline__ void load_row32(const T* p, uint32_t (&v)[16], int n,
   }
 }
 
-// The same 32 values of column group 0 or 1 of 64 into the warp's `out`, in the 128-byte
-// swizzle that the store's map names.  A store of whole 128-byte lines by the copy engine:
-// stores by lane, each to a row of its own, held up the epilogue (dg and du of 46080 x 2048:
-// 281 us against 2xx).
-__device__ __forceinline__ void put32(unsigned char* out, int lane, int group, const uint32_t (&v)[16]) {
+// ------------------------------------------------------------------ the way out
+//
+// A warp's 32 rows x 128 bytes go through its `out` and leave by whole rows: by the copy
+// engine where the matrix's rows start on 16 bytes, by coalesced stores elsewhere.
+// (Stores by lane, each to a row of its own, held up the epilogue.)
+
+// Values of this lane's row into `out`: 16-byte piece q of the row at q ^ (row mod 8), the
+// 128-byte swizzle that the store's map names.
+template <int N>
+__device__ __forceinline__ void put(unsigned char* out, int lane, int first, const uint32_t (&v)[N]) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q)
-    *reinterpret_cast<uint4*>(out + lane * 128 + (((group * 4 + q) ^ (lane & 7)) << 4)) =
+  for (int q = 0; q < N / 4; ++q)
+    *reinterpret_cast<uint4*>(out + lane * 128 + (((first + q) ^ (lane & 7)) << 4)) =
         make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
 }
 // `out` is free again: its last store has been read out of it (all lanes).
@@ -486,8 +472,7 @@ __device__ __forceinline__ void out_free(int lane) {
   if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   __syncwarp();
 }
-// 64 columns x 32 rows of `out` to (col, row) (all lanes; rows and columns past the map's
-// end are left out).
+// `out` to (col, row) of a map (all lanes; rows and columns past its end are left out).
 __device__ __forceinline__ void out_store(const unsigned char* out, const CUtensorMap* map, int col, int row, int lane) {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
@@ -498,6 +483,30 @@ __device__ __forceinline__ void out_store(const unsigned char* out, const CUtens
                  : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
   }
+}
+
+// `out` to the matrix at p, `ld` elements of SIZE bytes between its rows; `rows` rows and
+// `cols` columns exist.
+template <int SIZE>
+__device__ __forceinline__ void out_rows(const unsigned char* out, void* p, int64_t ld, int rows, int cols, int lane) {
+  __syncwarp();
+  char* q = static_cast<char*>(p);
+  const bool words = SIZE == 4 || (ld % 2 == 0 && (reinterpret_cast<uintptr_t>(p) & 3) == 0);
+  const int c = SIZE == 4 ? lane : 2 * lane;  // of the lane's word
+  for (int r = 0; r < min(rows, 32); ++r) {
+    const uint32_t w =
+        *reinterpret_cast<const uint32_t*>(out + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+    char* at = q + (r * ld + c) * SIZE;
+    if constexpr (SIZE == 4) {
+      if (c < cols) *reinterpret_cast<uint32_t*>(at) = w;
+    } else if (words && c + 1 < cols) {
+      *reinterpret_cast<uint32_t*>(at) = w;
+    } else {
+      if (c < cols) *reinterpret_cast<uint16_t*>(at) = (uint16_t)w;
+      if (c + 1 < cols) *reinterpret_cast<uint16_t*>(at + 2) = (uint16_t)(w >> 16);
+    }
+  }
+  __syncwarp();
 }
 
 // ------------------------------------------------------------------ host side

@@ -30,8 +30,8 @@ struct HiddenEpi {
     T *o0, *o1;          // h, or dg and du
     int64_t rows;
     int hidden, ldo;     // columns; elements between the rows of the outputs
-    int wide, wide_dh;   // rows start on 32 bytes
-    int mapped;          // rows start on 16 bytes, as the copy engine's stores ask
+    int ldd;             // and of dh
+    int mapped;          // the outputs' rows start on 16 bytes, as the copy engine asks
   };
   static __host__ __device__ constexpr int GROUPS(int BN) { return BN >= 128 ? BN / 128 : 1; }  // of 32 columns of a warp
   // The cotangents of a warp's columns, on their way while the products run.
@@ -46,7 +46,7 @@ struct HiddenEpi {
       for (int k = 0; k < GROUPS(BN); ++k) {
         const int c = half * GROUPS(BN) + k, col = t.n * (BN / 2) + c * 32;
         const int n = row < p.rows && c < BN / 64 ? p.hidden - col : 0;
-        gemm::load_row32(p.dh + row * p.hidden + col, f.d[k], n, p.wide_dh);
+        gemm::load_row32(p.dh + row * p.ldd + col, f.d[k], n);
       }
     }
   }
@@ -54,7 +54,6 @@ struct HiddenEpi {
   static __device__ __forceinline__ void run(const Params& p, const Tile& t, int64_t row, int half, uint32_t addr,
                                              const Ahead<BN>& f, unsigned char* out, Release release) {
     const int lane = threadIdx.x & 31;
-    const bool mapped = GROUPS(BN) == 2 && p.mapped;  // 64 columns: whole lines
     const int col0 = t.n * (BN / 2) + half * GROUPS(BN) * 32;
     uint32_t keep[GROUPS(BN)][16];
 #pragma unroll
@@ -87,25 +86,22 @@ struct HiddenEpi {
           o[i] = gemm::pack2<T>(x.x, x.y);
         }
       }
-      if (mapped) {
-        if (k == 0) gemm::out_free(lane);
-        gemm::put32(out, lane, k, o);
-      } else {
-        const int col = col0 + k * 32, n = row < p.rows ? p.hidden - col : 0;
-        if (n > 0) {
-          gemm::store_row32(p.o0 + row * p.ldo + col, o, n, p.wide);
-          if (BWD) gemm::store_row32(p.o1 + row * p.ldo + col, keep[k], n, p.wide);
-        }
-      }
+      if (k == 0) gemm::out_free(lane);
+      gemm::put(out, lane, 4 * k, o);
     }
-    const int64_t row0 = row - lane;
-    if (!mapped || col0 >= p.hidden || row0 >= p.rows) return;
-    gemm::out_store(out, &p.m0, col0, (int)row0, lane);
+    const int row0 = (int)(row - lane);
+    const int rows = (int)min(p.rows - row0, (int64_t)32), cols = min(p.hidden - col0, 32 * GROUPS(BN));
+    if (cols <= 0 || rows <= 0 || half * GROUPS(BN) >= BN / 64) return;
+    auto leave = [&](const CUtensorMap* m, T* o) {
+      if (GROUPS(BN) == 2 && p.mapped) gemm::out_store(out, m, col0, row0, lane);
+      else gemm::out_rows<2>(out, o + (int64_t)row0 * p.ldo + col0, p.ldo, rows, cols, lane);
+    };
+    leave(&p.m0, p.o0);
     if (BWD) {
       gemm::out_free(lane);
 #pragma unroll
-      for (int k = 0; k < GROUPS(BN); ++k) gemm::put32(out, lane, k, keep[k]);
-      gemm::out_store(out, &p.m1, col0, (int)row0, lane);
+      for (int k = 0; k < GROUPS(BN); ++k) gemm::put(out, lane, 4 * k, keep[k]);
+      leave(&p.m1, p.o1);
     }
   }
 };
@@ -121,7 +117,8 @@ struct StoreEpi {
     float* part;
     int64_t rows, pad;
     int cols;
-    int wide, mapped;
+    int wide;            // rows of `part` start on 16 bytes
+    int mapped;
   };
   template <int BN>
   struct Ahead {};
@@ -165,13 +162,14 @@ struct StoreEpi {
         uint32_t o[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i] = gemm::pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-        if (p.mapped) {
-          if ((c & 1) == 0) gemm::out_free(lane);
-          gemm::put32(stage, lane, c & 1, o);
-          if ((c & 1) && col - 32 < p.cols && row - lane < p.rows)
-            gemm::out_store(stage, map, col - 32, (int)(row - lane), lane);
-        } else if (n > 0) {
-          gemm::store_row32(out + row * p.cols + col, o, n, p.wide);
+        if ((c & 1) == 0) gemm::out_free(lane);
+        gemm::put(stage, lane, 4 * (c & 1), o);
+        const int64_t row0 = row - lane;
+        if ((c & 1) && col - 32 < p.cols && row0 < p.rows) {
+          if (p.mapped) gemm::out_store(stage, map, col - 32, (int)row0, lane);
+          else
+            gemm::out_rows<2>(stage, out + row0 * p.cols + col - 32, p.cols, (int)min(p.rows - row0, (int64_t)32),
+                              min(p.cols - col + 32, 64), lane);
         }
       }
     }
@@ -207,11 +205,16 @@ __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits
 }
 
 // Rows of `dim` elements copied to rows `ld` apart, for operands whose rows do not
-// start on 16 bytes as TMA asks.
-__global__ void __launch_bounds__(256) pitch_kernel(const uint16_t* src, int64_t rows, int dim, uint16_t* dst, int ld) {
-  const int64_t n = rows * dim;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-    dst[i / dim * ld + i % dim] = src[i];
+// start where TMA or a vector load asks; a warp per row.  W: one element or two.
+template <typename W>
+__global__ void __launch_bounds__(256) pitch_kernel(const W* src, int64_t rows, int n, W* dst, int ld) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
+    const W* a = src + r * n;
+    W* b = dst + r * ld;
+#pragma unroll 4
+    for (int c = lane; c < n; c += 32) b[c] = a[c];
+  }
 }
 
 struct Args {
@@ -239,7 +242,7 @@ static int weight_splits(int64_t rows, int dim, int hidden) {
 }
 
 struct Space {
-  size_t x, wg, wu, dg, du, part, total;
+  size_t x, wg, wu, dh, dg, du, part, total;
   int ldd, ldh, splits;
 };
 // Offsets of the workspace.  The padded copies have their place whenever the width
@@ -247,7 +250,7 @@ struct Space {
 static Space space(int64_t rows, int dim, int hidden, bool bwd) {
   Space s{};
   s.ldd = (int)up(dim, 8);
-  s.ldh = (int)up(hidden, 8);
+  s.ldh = (int)up(hidden, 16);  // 32 bytes, for vector loads of dh
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t o = at;
@@ -258,6 +261,7 @@ static Space space(int64_t rows, int dim, int hidden, bool bwd) {
   s.wg = take((size_t)hidden * s.ldd * 2);
   s.wu = take((size_t)hidden * s.ldd * 2);
   if (bwd) {
+    s.dh = take((size_t)rows * s.ldh * 2);
     s.dg = take((size_t)rows * s.ldh * 2);
     s.du = take((size_t)rows * s.ldh * 2);
     s.splits = weight_splits(rows, dim, hidden);
@@ -269,18 +273,22 @@ static Space space(int64_t rows, int dim, int hidden, bool bwd) {
 
 static bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-// The operand with rows that TMA can read: as it is, or copied.
-static const void* pitched(const void* p, int64_t rows, int dim, int ld, char* copy, cudaStream_t s) {
-  if (dim == ld && aligned(p, 16)) return p;
-  int64_t b = tiles(rows * dim, 256 * 8);
-  if (b > 148 * 16) b = 148 * 16;
-  pitch_kernel<<<(unsigned)b, 256, 0, s>>>((const uint16_t*)p, rows, dim, (uint16_t*)copy, ld);
+// The operand with rows that start on `align` bytes: as it is, or copied to rows of ld
+// elements.
+static const void* pitched(const void* p, int64_t rows, int dim, int ld, int align, char* copy, cudaStream_t s) {
+  if (dim == ld && aligned(p, align)) return p;
+  int64_t b = tiles(rows, 8);
+  if (b > device_sm_count() * 8) b = device_sm_count() * 8;
+  if (dim % 2 == 0 && aligned(p, 4))
+    pitch_kernel<uint32_t><<<(unsigned)b, 256, 0, s>>>((const uint32_t*)p, rows, dim / 2, (uint32_t*)copy, ld / 2);
+  else
+    pitch_kernel<uint16_t><<<(unsigned)b, 256, 0, s>>>((const uint16_t*)p, rows, dim, (uint16_t*)copy, ld);
   return copy;
 }
 
 template <typename T, int ACT, bool BWD, int CG, int BN>
-static cudaError_t hidden_pass(int dtype, const void* x, const void* wg, const void* wu, int ldd, const Args& p, T* o0,
-                               T* o1, int ldo, cudaStream_t s) {
+static cudaError_t hidden_pass(int dtype, const void* x, const void* wg, const void* wu, int ldd,
+                               const void* dh, int ldd_dh, const Args& p, T* o0, T* o1, int ldo, cudaStream_t s) {
   CUtensorMap a, b0, b1;
   const int box = BN / 2;
   if (!gemm::make_map(&a, dtype, x, p.dim, p.rows, (int64_t)ldd * 2, 128) ||
@@ -294,14 +302,13 @@ static cudaError_t hidden_pass(int dtype, const void* x, const void* wg, const v
   w.kb = (int)tiles(p.dim, 64);
   w.idesc = gemm::idesc_f16(dtype, 128 * CG, BN, false, false);
   typename HiddenEpi<T, ACT, BWD>::Params e{};
-  e.dh = (const T*)p.dh;
+  e.dh = (const T*)dh;
   e.o0 = o0;
   e.o1 = o1;
   e.rows = p.rows;
   e.hidden = p.hidden;
   e.ldo = ldo;
-  e.wide = ldo % 16 == 0 && aligned(o0, 32) && (!BWD || aligned(o1, 32));
-  e.wide_dh = p.hidden % 16 == 0 && aligned(p.dh, 32);
+  e.ldd = ldd_dh;
   e.mapped = BN == 256 && ldo % 8 == 0 && aligned(o0, 16) && (!BWD || aligned(o1, 16)) &&
              gemm::make_map(&e.m0, dtype, o0, p.hidden, p.rows, (int64_t)ldo * 2, 32) &&
              (!BWD || gemm::make_map(&e.m1, dtype, o1, p.hidden, p.rows, (int64_t)ldo * 2, 32));
@@ -310,9 +317,9 @@ static cudaError_t hidden_pass(int dtype, const void* x, const void* wg, const v
 }
 
 template <typename T, int ACT, bool BWD>
-static cudaError_t hidden_any(int dtype, const void* x, const void* wg, const void* wu, int ldd, const Args& p, T* o0,
-                              T* o1, int ldo, cudaStream_t s) {
-  return hidden_pass<T, ACT, BWD, 2, 256>(dtype, x, wg, wu, ldd, p, o0, o1, ldo, s);
+static cudaError_t hidden_any(int dtype, const void* x, const void* wg, const void* wu, int ldd, const void* dh,
+                              int ldd_dh, const Args& p, T* o0, T* o1, int ldo, cudaStream_t s) {
+  return hidden_pass<T, ACT, BWD, 2, 256>(dtype, x, wg, wu, ldd, dh, ldd_dh, p, o0, o1, ldo, s);
 }
 
 // dx = dg Wg + du Wu: the weights as they lie are the second operand with its rows
@@ -337,7 +344,6 @@ static cudaError_t input_gradient(int dtype, const T* dg, const T* du, const voi
   e.o0 = (T*)p.dx;
   e.rows = p.rows;
   e.cols = p.dim;
-  e.wide = p.dim % 16 == 0 && aligned(p.dx, 32);
   e.mapped = p.dim % 8 == 0 && aligned(p.dx, 16) && gemm::make_map(&e.m0, dtype, p.dx, p.dim, p.rows, (int64_t)p.dim * 2, 32);
   return gemm::launch<gemm::OP_SUM, 2, 256, false, true, false, StoreEpi<T, false>>(a0, a1, b0, b1, w, e,
                                                                                     device_sm_count(), s);
@@ -366,7 +372,7 @@ static cudaError_t weight_gradients(int dtype, const T* dg, const T* du, const v
   e.rows = p.hidden;
   e.pad = (int64_t)w.mt0 * 256;
   e.cols = p.dim;
-  e.wide = e.part ? p.dim % 4 == 0 : p.dim % 16 == 0 && aligned(p.dwg, 32) && aligned(p.dwu, 32);
+  e.wide = p.dim % 4 == 0;
   e.mapped = !e.part && p.dim % 8 == 0 && p.dwg && p.dwu && aligned(p.dwg, 16) && aligned(p.dwu, 16) &&
              gemm::make_map(&e.m0, dtype, p.dwg, p.dim, p.hidden, (int64_t)p.dim * 2, 32) &&
              gemm::make_map(&e.m1, dtype, p.dwu, p.dim, p.hidden, (int64_t)p.dim * 2, 32);
@@ -383,12 +389,13 @@ static cudaError_t weight_gradients(int dtype, const T* dg, const T* du, const v
 template <typename T, int ACT>
 static cudaError_t run(int dtype, const Args& p, bool bwd, cudaStream_t s) {
   const Space L = space(p.rows, p.dim, p.hidden, bwd);
-  const void* x = pitched(p.x, p.rows, p.dim, L.ldd, p.ws + L.x, s);
-  const void* wg = pitched(p.wg, p.hidden, p.dim, L.ldd, p.ws + L.wg, s);
-  const void* wu = pitched(p.wu, p.hidden, p.dim, L.ldd, p.ws + L.wu, s);
-  if (!bwd) return hidden_any<T, ACT, false>(dtype, x, wg, wu, L.ldd, p, (T*)p.h, nullptr, p.hidden, s);
+  const void* x = pitched(p.x, p.rows, p.dim, L.ldd, 16, p.ws + L.x, s);
+  const void* wg = pitched(p.wg, p.hidden, p.dim, L.ldd, 16, p.ws + L.wg, s);
+  const void* wu = pitched(p.wu, p.hidden, p.dim, L.ldd, 16, p.ws + L.wu, s);
+  if (!bwd) return hidden_any<T, ACT, false>(dtype, x, wg, wu, L.ldd, nullptr, 0, p, (T*)p.h, nullptr, p.hidden, s);
+  const void* dh = pitched(p.dh, p.rows, p.hidden, L.ldh, 32, p.ws + L.dh, s);
   T *dg = (T*)(p.ws + L.dg), *du = (T*)(p.ws + L.du);
-  cudaError_t e = hidden_any<T, ACT, true>(dtype, x, wg, wu, L.ldd, p, dg, du, L.ldh, s);
+  cudaError_t e = hidden_any<T, ACT, true>(dtype, x, wg, wu, L.ldd, dh, L.ldh, p, dg, du, L.ldh, s);
   if (e == cudaSuccess && p.dx) e = input_gradient<T>(dtype, dg, du, wg, wu, L.ldd, L.ldh, p, s);
   if (e == cudaSuccess && (p.dwg || p.dwu))
     e = weight_gradients<T>(dtype, dg, du, x, L.ldd, L.ldh, L.splits, (float*)(p.ws + L.part), p, s);

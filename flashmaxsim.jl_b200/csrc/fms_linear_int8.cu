@@ -214,8 +214,7 @@ struct ScaleEpi {
     Y* y;
     int64_t rows;
     int cols;
-    int wide;         // rows of y start on 32 bytes
-    int mapped;       // 16-bit rows that start on 16 bytes, 64 columns to a warp
+    int mapped;       // rows of y start on 16 bytes
   };
   template <int BN>
   struct Ahead {};
@@ -233,7 +232,6 @@ struct ScaleEpi {
       gemm::load32(addr + c * 32, v);
       if (c + 1 == (half + 1) * (BN / 64)) release();
       const int col = t.n * BN + c * 32;
-      const int n = row < p.rows ? p.cols - col : 0;
       float f[32];
       // columns past the end take the last one's scale; they are not stored
 #pragma unroll
@@ -242,28 +240,28 @@ struct ScaleEpi {
         f[i] = (sx * __ldg(p.sw + at)) * (float)(int32_t)v[i];
         if (p.bias) f[i] += Tr<Y>::to(p.bias[at]);
       }
-      Y* out = p.y + row * p.cols + col;
+      // 128 bytes of a row at a time: every 32 columns in float32, every 64 in 16 bits
+      constexpr int PER = 128 / sizeof(Y), GROUPS = BN >= 128 ? PER / 32 : 1;
+      const int k = GROUPS == 2 ? c & 1 : 0;
+      if (k == 0) gemm::out_free(lane);
       if constexpr (sizeof(Y) == 2) {
         uint32_t o[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i] = gemm::pack2<Y>(f[2 * i], f[2 * i + 1]);
-        if (BN >= 128 && p.mapped) {
-          if ((c & 1) == 0) gemm::out_free(lane);
-          gemm::put32(stage, lane, c & 1, o);
-          if ((c & 1) && col - 32 < p.cols && row - lane < p.rows)
-            gemm::out_store(stage, &p.map, col - 32, (int)(row - lane), lane);
-        } else if (n > 0) {
-          gemm::store_row32(out, o, n, p.wide);
-        }
-      } else if (n > 0) {
-        uint32_t o[16];
+        gemm::put(stage, lane, 4 * k, o);
+      } else {
+        uint32_t o[32];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // 16 floats are 32 half-words
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(f[16 * h + i]);
-          if (n > 16 * h) gemm::store_row32(reinterpret_cast<uint16_t*>(out + 16 * h), o, 2 * (n - 16 * h), p.wide);
-        }
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(f[i]);
+        gemm::put(stage, lane, 0, o);
       }
+      const int col0 = col - 32 * k;
+      const int64_t row0 = row - lane;
+      if (k != GROUPS - 1 || col0 >= p.cols || row0 >= p.rows) continue;
+      if (32 * GROUPS == PER && p.mapped) gemm::out_store(stage, &p.map, col0, (int)row0, lane);
+      else
+        gemm::out_rows<sizeof(Y)>(stage, p.y + row0 * p.cols + col0, p.cols, (int)min(p.rows - row0, (int64_t)32),
+                                  min(p.cols - col0, 32 * GROUPS), lane);
     }
   }
 };
@@ -368,10 +366,9 @@ static cudaError_t product(const int8_t* xc, const float* sx, const int8_t* wc, 
   e.y = (Y*)p.y;
   e.rows = p.rows;
   e.cols = p.C;
-  e.wide = (p.C * sizeof(Y)) % 32 == 0 && aligned(p.y, 32);
-  e.mapped = sizeof(Y) == 2 && BN >= 128 && p.C % 8 == 0 && aligned(p.y, 16) &&
-             gemm::make_map(&e.map, std::is_same<Y, __half>::value ? FMS_F16 : FMS_BF16, p.y, p.C, p.rows,
-                            (int64_t)p.C * 2, 32);
+  e.mapped = p.C * sizeof(Y) % 16 == 0 && aligned(p.y, 16) &&
+             gemm::make_map(&e.map, sizeof(Y) == 4 ? FMS_F32 : std::is_same<Y, __half>::value ? FMS_F16 : FMS_BF16, p.y, p.C,
+                            p.rows, (int64_t)p.C * sizeof(Y), 32);
   return gemm::launch<gemm::OP_ONE, CG, BN, false, false, true, ScaleEpi<Y>>(a, a, b, b, w, e, device_sm_count(), s);
 }
 

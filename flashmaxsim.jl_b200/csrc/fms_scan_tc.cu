@@ -972,10 +972,11 @@ bool make_map(CUtensorMap* m, int dtype, const void* base, int64_t inner, int64_
   const bool i8 = dtype == FMS_I8;
   cuuint64_t gdim[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
   cuuint64_t gstride[1] = {(cuuint64_t)pitch};
-  cuuint32_t tile[2] = {i8 ? 128u : 64u, (cuuint32_t)box};
+  cuuint32_t tile[2] = {i8 ? 128u : dtype == FMS_F32 ? 32u : 64u, (cuuint32_t)box};
   cuuint32_t estride[2] = {1, 1};
-  const CUtensorMapDataType t = i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                                   : dtype == FMS_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+  const CUtensorMapDataType t = i8                 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                : dtype == FMS_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                : dtype == FMS_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   return enc(m, t, 2, const_cast<void*>(base), gdim, gstride, tile, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
