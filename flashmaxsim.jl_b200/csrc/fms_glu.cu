@@ -1,416 +1,14 @@
-// fms_glu.cu -- the gated feed-forward block of a token encoder:
-//
-//   g = x Wg^T,  u = x Wu^T,  h = a(g) * u                      (forward)
-//   du = dh * a(g),  dg = dh * u * a'(g)                        (backward)
-//   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
-//
-// x (rows, dim), Wg and Wu (hidden, dim), h (rows, hidden), 16-bit; sums in
-// float32.  One kernel makes both projections of a tile into one accumulator (its
-// columns are those of Wg and of Wu) and applies the activation and the product as
-// it leaves TMEM.  g and u are not kept for the backward pass but computed again by
-// the same kernel with another epilogue: one more pair of products, against rounding
-// g and u to 16 bits (which would double the gradients' error) and 4 * rows * hidden
-// bytes between the passes.  dg and du are rounded to the inputs' type, the type of
-// the products they enter.
-#include "fms_act.cuh"
-#include "fms_gemm_tc.cuh"
-#include "fms_internal.h"
+// fms_glu.cu -- entry points of the gated feed-forward block (fms_glu.cuh).
+#include "fms_glu.cuh"
 
 namespace fms {
+
+cudaError_t run_ffn_f16(int dtype, int act, const glu::Args& p, bool bwd, cudaStream_t s);
+cudaError_t run_ffn_bf16(int dtype, int act, const glu::Args& p, bool bwd, cudaStream_t s);
+int read_ffn_f16_error(int reset);
+int read_ffn_bf16_error(int reset);
+
 namespace glu {
-
-using gemm::Tile;
-
-// h = a(g) u, or with BWD dg = dh u a'(g) and du = dh a(g).
-template <typename T, int ACT, bool BWD>
-struct HiddenEpi {
-  struct alignas(64) Params {
-    CUtensorMap m0, m1;  // o0 and o1, where `mapped`
-    const T* dh;
-    T *o0, *o1;          // h, or dg and du
-    int64_t rows;
-    int hidden, ldo;     // columns; elements between the rows of the outputs
-    int ldd;             // and of dh
-    int mapped;          // the outputs' rows start on 16 bytes, as the copy engine asks
-  };
-  static __host__ __device__ constexpr int GROUPS(int BN) { return BN >= 128 ? BN / 128 : 1; }  // of 32 columns of a warp
-  // The cotangents of a warp's columns, on their way while the products run.
-  template <int BN>
-  struct Ahead {
-    uint32_t d[BWD ? GROUPS(BN) : 1][16];
-  };
-  template <int BN>
-  static __device__ __forceinline__ void fetch(const Params& p, const Tile& t, int64_t row, int half, Ahead<BN>& f) {
-    if constexpr (BWD) {
-#pragma unroll
-      for (int k = 0; k < GROUPS(BN); ++k) {
-        const int c = half * GROUPS(BN) + k, col = t.n * (BN / 2) + c * 32;
-        const int n = row < p.rows && c < BN / 64 ? p.hidden - col : 0;
-        gemm::load_row32(p.dh + row * p.ldd + col, f.d[k], n);
-      }
-    }
-  }
-  template <int BN, class Release>
-  static __device__ __forceinline__ void run(const Params& p, const Tile& t, int64_t row, int half, uint32_t addr,
-                                             const Ahead<BN>& f, unsigned char* out, Release release) {
-    const int lane = threadIdx.x & 31;
-    const int col0 = t.n * (BN / 2) + half * GROUPS(BN) * 32;
-    uint32_t keep[GROUPS(BN)][16];
-#pragma unroll
-    for (int k = 0; k < GROUPS(BN); ++k) {
-      const int c = half * GROUPS(BN) + k;
-      if (c >= BN / 64) {
-        release();
-        break;
-      }
-      __syncwarp();
-      uint32_t g[32], u[32];
-      ptx::tmem_ld32(addr + c * 32, g);
-      gemm::load32(addr + BN / 2 + c * 32, u);  // waits for both
-      gemm::landed(g);
-      if (k == GROUPS(BN) - 1) release();
-      uint32_t o[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float2 a, da;
-        const float2 gv = make_float2(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
-        const float2 uv = make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
-        act_eval2<ACT, BWD>(gv, a, da);
-        if (BWD) {
-          const float2 e = gemm::unpack2<T>(f.d[k][i]);
-          const float2 x = __fmul2_rn(__fmul2_rn(e, uv), da), y = __fmul2_rn(e, a);
-          o[i] = gemm::pack2<T>(x.x, x.y);
-          keep[k][i] = gemm::pack2<T>(y.x, y.y);
-        } else {
-          const float2 x = __fmul2_rn(a, uv);
-          o[i] = gemm::pack2<T>(x.x, x.y);
-        }
-      }
-      if (k == 0) gemm::out_free(lane);
-      gemm::put(out, lane, 4 * k, o);
-    }
-    const int row0 = (int)(row - lane);
-    const int rows = (int)min(p.rows - row0, (int64_t)32), cols = min(p.hidden - col0, 32 * GROUPS(BN));
-    if (cols <= 0 || rows <= 0 || half * GROUPS(BN) >= BN / 64) return;
-    auto leave = [&](const CUtensorMap* m, T* o) {
-      if (GROUPS(BN) == 2 && p.mapped) gemm::out_store(out, m, col0, row0, lane);
-      else gemm::out_rows<2>(out, o + (int64_t)row0 * p.ldo + col0, p.ldo, rows, cols, lane);
-    };
-    leave(&p.m0, p.o0);
-    if (BWD) {
-      gemm::out_free(lane);
-#pragma unroll
-      for (int k = 0; k < GROUPS(BN); ++k) gemm::put(out, lane, 4 * k, keep[k]);
-      leave(&p.m1, p.o1);
-    }
-  }
-};
-
-// The accumulator as it is, in T, or in float32 where the sum is split (`part` then
-// holds one (rows, cols) matrix after the other).  STACK: the rows are those of two
-// outputs, `pad` rows of tiles each.
-template <typename T, bool STACK>
-struct StoreEpi {
-  struct alignas(64) Params {
-    CUtensorMap m0, m1;  // o0 and o1, where `mapped`
-    T *o0, *o1;
-    float* part;
-    int64_t rows, pad;
-    int cols;
-    int wide;            // rows of `part` start on 16 bytes
-    int mapped;
-  };
-  template <int BN>
-  struct Ahead {};
-  template <int BN>
-  static __device__ __forceinline__ void fetch(const Params&, const Tile&, int64_t, int, Ahead<BN>&) {}
-  template <int BN, class Release>
-  static __device__ __forceinline__ void run(const Params& p, const Tile& t, int64_t row, int half, uint32_t addr,
-                                             const Ahead<BN>&, unsigned char* stage, Release release) {
-    static_assert(BN >= 128, "64 columns to a warp");
-    const int lane = threadIdx.x & 31;
-    T* out = p.o0;
-    const CUtensorMap* map = &p.m0;
-    int64_t at = t.split * (STACK ? 2 : 1) * p.rows;
-    if (STACK && row >= p.pad) {
-      row -= p.pad;
-      out = p.o1;
-      map = &p.m1;
-      at += p.rows;
-    }
-#pragma unroll 1
-    for (int c = half * (BN / 64); c < (half + 1) * (BN / 64); ++c) {
-      __syncwarp();
-      uint32_t v[32];
-      gemm::load32(addr + c * 32, v);
-      if (c + 1 == (half + 1) * (BN / 64)) release();
-      const int col = t.n * BN + c * 32;
-      const int n = row < p.rows ? p.cols - col : 0;
-      if (p.part) {
-        if (n <= 0) continue;
-        float* q = p.part + (at + row) * p.cols + col;
-        if (n >= 32 && p.wide) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            reinterpret_cast<uint4*>(q)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (i < n) q[i] = __uint_as_float(v[i]);
-        }
-      } else if (out) {
-        uint32_t o[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = gemm::pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-        if ((c & 1) == 0) gemm::out_free(lane);
-        gemm::put(stage, lane, 4 * (c & 1), o);
-        const int64_t row0 = row - lane;
-        if ((c & 1) && col - 32 < p.cols && row0 < p.rows) {
-          if (p.mapped) gemm::out_store(stage, map, col - 32, (int)row0, lane);
-          else
-            gemm::out_rows<2>(stage, out + row0 * p.cols + col - 32, p.cols, (int)min(p.rows - row0, (int64_t)32),
-                              min(p.cols - col + 32, 64), lane);
-        }
-      }
-    }
-  }
-};
-
-// Sum of the parts of a split product, in order.
-template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int64_t each, T* o0, T* o1) {
-  const int64_t n = 2 * each;
-  if (each % 4 == 0 && ((reinterpret_cast<uintptr_t>(o0) | reinterpret_cast<uintptr_t>(o1)) & 7) == 0) {
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
-      T* o = i < each ? o0 : o1;
-      if (!o) continue;
-      float4 s = *reinterpret_cast<const float4*>(part + i);
-#pragma unroll 4
-      for (int k = 1; k < splits; ++k) {
-        const float4 v = *reinterpret_cast<const float4*>(part + k * n + i);
-        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-      }
-      *reinterpret_cast<uint2*>(o + (i < each ? i : i - each)) =
-          make_uint2(gemm::pack2<T>(s.x, s.y), gemm::pack2<T>(s.z, s.w));
-    }
-    return;
-  }
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    T* o = i < each ? o0 : o1;
-    if (!o) continue;
-    float s = part[i];
-    for (int k = 1; k < splits; ++k) s += part[k * n + i];
-    o[i < each ? i : i - each] = Tr<T>::from(s);
-  }
-}
-
-// Rows of `dim` elements copied to rows `ld` apart, for operands whose rows do not
-// start where TMA or a vector load asks; a warp per row.  W: one element or two.
-template <typename W>
-__global__ void __launch_bounds__(256) pitch_kernel(const W* src, int64_t rows, int n, W* dst, int ld) {
-  const int lane = threadIdx.x & 31;
-  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
-    const W* a = src + r * n;
-    W* b = dst + r * ld;
-#pragma unroll 4
-    for (int c = lane; c < n; c += 32) b[c] = a[c];
-  }
-}
-
-struct Args {
-  const void *x, *wg, *wu, *dh;
-  int64_t rows;
-  int dim, hidden;
-  void *h, *dx, *dwg, *dwu;
-  char* ws;
-};
-
-static int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
-static int64_t tiles(int64_t n, int64_t t) { return (n + t - 1) / t; }
-
-// Parts of the sum over rows for the weights' gradients: enough to give every pair of
-// SMs a tile of about the same length, at least 16 blocks of 64 rows each.
-static int weight_splits(int64_t rows, int dim, int hidden) {
-  const int64_t t = 2 * tiles(hidden, 256) * tiles(dim, 256), pairs = device_sm_count() / 2, kb = tiles(rows, 64);
-  int64_t best = 1;
-  double cost = 1e30;
-  for (int64_t s = 1; s <= 16 && (s == 1 || kb / s >= 16); ++s) {
-    const double c = (double)tiles(t * s, pairs) * ((double)kb / s + 8.0);  // + a tile's start and end
-    if (c < cost * 0.97) cost = c, best = s;
-  }
-  return (int)best;
-}
-
-struct Space {
-  size_t x, wg, wu, dh, dg, du, part, total;
-  int ldd, ldh, splits;
-};
-// Offsets of the workspace.  The padded copies have their place whenever the width
-// asks for them or a pointer might (the size is known without the pointers).
-static Space space(int64_t rows, int dim, int hidden, bool bwd) {
-  Space s{};
-  s.ldd = (int)up(dim, 8);
-  s.ldh = (int)up(hidden, 16);  // 32 bytes, for vector loads of dh
-  size_t at = 0;
-  auto take = [&](size_t n) {
-    const size_t o = at;
-    at += (size_t)up((int64_t)n, 256);
-    return o;
-  };
-  s.x = take((size_t)rows * s.ldd * 2);
-  s.wg = take((size_t)hidden * s.ldd * 2);
-  s.wu = take((size_t)hidden * s.ldd * 2);
-  if (bwd) {
-    s.dh = take((size_t)rows * s.ldh * 2);
-    s.dg = take((size_t)rows * s.ldh * 2);
-    s.du = take((size_t)rows * s.ldh * 2);
-    s.splits = weight_splits(rows, dim, hidden);
-    if (s.splits > 1) s.part = take((size_t)s.splits * 2 * hidden * dim * 4);
-  }
-  s.total = at;
-  return s;
-}
-
-static bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-
-// The operand with rows that start on `align` bytes: as it is, or copied to rows of ld
-// elements.
-static const void* pitched(const void* p, int64_t rows, int dim, int ld, int align, char* copy, cudaStream_t s) {
-  if (dim == ld && aligned(p, align)) return p;
-  int64_t b = tiles(rows, 8);
-  if (b > device_sm_count() * 8) b = device_sm_count() * 8;
-  if (dim % 2 == 0 && aligned(p, 4))
-    pitch_kernel<uint32_t><<<(unsigned)b, 256, 0, s>>>((const uint32_t*)p, rows, dim / 2, (uint32_t*)copy, ld / 2);
-  else
-    pitch_kernel<uint16_t><<<(unsigned)b, 256, 0, s>>>((const uint16_t*)p, rows, dim, (uint16_t*)copy, ld);
-  return copy;
-}
-
-template <typename T, int ACT, bool BWD, int CG, int BN>
-static cudaError_t hidden_pass(int dtype, const void* x, const void* wg, const void* wu, int ldd,
-                               const void* dh, int ldd_dh, const Args& p, T* o0, T* o1, int ldo, cudaStream_t s) {
-  CUtensorMap a, b0, b1;
-  const int box = BN / 2;
-  if (!gemm::make_map(&a, dtype, x, p.dim, p.rows, (int64_t)ldd * 2, 128) ||
-      !gemm::make_map(&b0, dtype, wg, p.dim, p.hidden, (int64_t)ldd * 2, box) ||
-      !gemm::make_map(&b1, dtype, wu, p.dim, p.hidden, (int64_t)ldd * 2, box))
-    return cudaErrorNotSupported;
-  gemm::Work w{};
-  w.mt = (int)tiles(p.rows, 128 * CG);
-  w.nt = (int)tiles(p.hidden, BN / 2);
-  w.splits = 1;
-  w.kb = (int)tiles(p.dim, 64);
-  w.idesc = gemm::idesc_f16(dtype, 128 * CG, BN, false, false);
-  typename HiddenEpi<T, ACT, BWD>::Params e{};
-  e.dh = (const T*)dh;
-  e.o0 = o0;
-  e.o1 = o1;
-  e.rows = p.rows;
-  e.hidden = p.hidden;
-  e.ldo = ldo;
-  e.ldd = ldd_dh;
-  e.mapped = BN == 256 && ldo % 8 == 0 && aligned(o0, 16) && (!BWD || aligned(o1, 16)) &&
-             gemm::make_map(&e.m0, dtype, o0, p.hidden, p.rows, (int64_t)ldo * 2, 32) &&
-             (!BWD || gemm::make_map(&e.m1, dtype, o1, p.hidden, p.rows, (int64_t)ldo * 2, 32));
-  return gemm::launch<gemm::OP_PAIR_B, CG, BN, false, false, false, HiddenEpi<T, ACT, BWD>>(a, a, b0, b1, w, e,
-                                                                                            device_sm_count(), s);
-}
-
-template <typename T, int ACT, bool BWD>
-static cudaError_t hidden_any(int dtype, const void* x, const void* wg, const void* wu, int ldd, const void* dh,
-                              int ldd_dh, const Args& p, T* o0, T* o1, int ldo, cudaStream_t s) {
-  return hidden_pass<T, ACT, BWD, 2, 256>(dtype, x, wg, wu, ldd, dh, ldd_dh, p, o0, o1, ldo, s);
-}
-
-// dx = dg Wg + du Wu: the weights as they lie are the second operand with its rows
-// along the sum.
-template <typename T>
-static cudaError_t input_gradient(int dtype, const T* dg, const T* du, const void* wg, const void* wu, int ldd, int ldh,
-                                  const Args& p, cudaStream_t s) {
-  CUtensorMap a0, a1, b0, b1;
-  if (!gemm::make_map(&a0, dtype, dg, p.hidden, p.rows, (int64_t)ldh * 2, 128) ||
-      !gemm::make_map(&a1, dtype, du, p.hidden, p.rows, (int64_t)ldh * 2, 128) ||
-      !gemm::make_map(&b0, dtype, wg, p.dim, p.hidden, (int64_t)ldd * 2, 64) ||
-      !gemm::make_map(&b1, dtype, wu, p.dim, p.hidden, (int64_t)ldd * 2, 64))
-    return cudaErrorNotSupported;
-  gemm::Work w{};
-  w.mt = (int)tiles(p.rows, 256);
-  w.nt = (int)tiles(p.dim, 256);
-  w.splits = 1;
-  w.kb0 = (int)tiles(p.hidden, 64);
-  w.kb = 2 * w.kb0;
-  w.idesc = gemm::idesc_f16(dtype, 256, 256, false, true);
-  typename StoreEpi<T, false>::Params e{};
-  e.o0 = (T*)p.dx;
-  e.rows = p.rows;
-  e.cols = p.dim;
-  e.mapped = p.dim % 8 == 0 && aligned(p.dx, 16) && gemm::make_map(&e.m0, dtype, p.dx, p.dim, p.rows, (int64_t)p.dim * 2, 32);
-  return gemm::launch<gemm::OP_SUM, 2, 256, false, true, false, StoreEpi<T, false>>(a0, a1, b0, b1, w, e,
-                                                                                    device_sm_count(), s);
-}
-
-// dWg = dg^T x over dWu = du^T x: both operands have their rows along the sum.
-template <typename T>
-static cudaError_t weight_gradients(int dtype, const T* dg, const T* du, const void* x, int ldd, int ldh, int splits,
-                                    float* part, const Args& p, cudaStream_t s) {
-  CUtensorMap a0, a1, b;
-  if (!gemm::make_map(&a0, dtype, dg, p.hidden, p.rows, (int64_t)ldh * 2, 64) ||
-      !gemm::make_map(&a1, dtype, du, p.hidden, p.rows, (int64_t)ldh * 2, 64) ||
-      !gemm::make_map(&b, dtype, x, p.dim, p.rows, (int64_t)ldd * 2, 64))
-    return cudaErrorNotSupported;
-  gemm::Work w{};
-  w.mt0 = (int)tiles(p.hidden, 256);
-  w.mt = 2 * w.mt0;
-  w.nt = (int)tiles(p.dim, 256);
-  w.splits = splits;
-  w.kb = (int)tiles(p.rows, 64);
-  w.idesc = gemm::idesc_f16(dtype, 256, 256, true, true);
-  typename StoreEpi<T, true>::Params e{};
-  e.o0 = (T*)p.dwg;
-  e.o1 = (T*)p.dwu;
-  e.part = splits > 1 ? part : nullptr;
-  e.rows = p.hidden;
-  e.pad = (int64_t)w.mt0 * 256;
-  e.cols = p.dim;
-  e.wide = p.dim % 4 == 0;
-  e.mapped = !e.part && p.dim % 8 == 0 && p.dwg && p.dwu && aligned(p.dwg, 16) && aligned(p.dwu, 16) &&
-             gemm::make_map(&e.m0, dtype, p.dwg, p.dim, p.hidden, (int64_t)p.dim * 2, 32) &&
-             gemm::make_map(&e.m1, dtype, p.dwu, p.dim, p.hidden, (int64_t)p.dim * 2, 32);
-  const cudaError_t err = gemm::launch<gemm::OP_STACK_A, 2, 256, true, true, false, StoreEpi<T, true>>(
-      a0, a1, b, b, w, e, device_sm_count(), s);
-  if (err != cudaSuccess || splits == 1) return err;
-  const int64_t each = (int64_t)p.hidden * p.dim;
-  int64_t blocks = tiles(2 * each, 256 * 4);
-  if (blocks > device_sm_count() * 8) blocks = device_sm_count() * 8;
-  join_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(part, splits, each, (T*)p.dwg, (T*)p.dwu);
-  return cudaGetLastError();
-}
-
-template <typename T, int ACT>
-static cudaError_t run(int dtype, const Args& p, bool bwd, cudaStream_t s) {
-  const Space L = space(p.rows, p.dim, p.hidden, bwd);
-  const void* x = pitched(p.x, p.rows, p.dim, L.ldd, 16, p.ws + L.x, s);
-  const void* wg = pitched(p.wg, p.hidden, p.dim, L.ldd, 16, p.ws + L.wg, s);
-  const void* wu = pitched(p.wu, p.hidden, p.dim, L.ldd, 16, p.ws + L.wu, s);
-  if (!bwd) return hidden_any<T, ACT, false>(dtype, x, wg, wu, L.ldd, nullptr, 0, p, (T*)p.h, nullptr, p.hidden, s);
-  const void* dh = pitched(p.dh, p.rows, p.hidden, L.ldh, 32, p.ws + L.dh, s);
-  T *dg = (T*)(p.ws + L.dg), *du = (T*)(p.ws + L.du);
-  cudaError_t e = hidden_any<T, ACT, true>(dtype, x, wg, wu, L.ldd, dh, L.ldh, p, dg, du, L.ldh, s);
-  if (e == cudaSuccess && p.dx) e = input_gradient<T>(dtype, dg, du, wg, wu, L.ldd, L.ldh, p, s);
-  if (e == cudaSuccess && (p.dwg || p.dwu))
-    e = weight_gradients<T>(dtype, dg, du, x, L.ldd, L.ldh, L.splits, (float*)(p.ws + L.part), p, s);
-  return e;
-}
-
-template <typename T>
-static cudaError_t run_act(int dtype, int act, const Args& p, bool bwd, cudaStream_t s) {
-  switch (act) {
-    case FMS_ACT_SILU: return run<T, FMS_ACT_SILU>(dtype, p, bwd, s);
-    case FMS_ACT_GELU: return run<T, FMS_ACT_GELU>(dtype, p, bwd, s);
-    case FMS_ACT_GELU_TANH: return run<T, FMS_ACT_GELU_TANH>(dtype, p, bwd, s);
-    default: return run<T, FMS_ACT_RELU>(dtype, p, bwd, s);
-  }
-}
 
 static int check(int dtype, int act, int64_t rows, int dim, int hidden) {
   if (dtype != FMS_F16 && dtype != FMS_BF16) return FMS_ERR_DTYPE;
@@ -423,14 +21,16 @@ static int check(int dtype, int act, int64_t rows, int dim, int hidden) {
 
 static int launch(int dtype, int act, const Args& p, bool bwd, cudaStream_t s) {
   if (device_cc() != 100) return FMS_ERR_UNSUPPORTED;
-  const cudaError_t e =
-      dtype == FMS_F16 ? run_act<__half>(dtype, act, p, bwd, s) : run_act<__nv_bfloat16>(dtype, act, p, bwd, s);
+  const cudaError_t e = dtype == FMS_F16 ? run_ffn_f16(dtype, act, p, bwd, s) : run_ffn_bf16(dtype, act, p, bwd, s);
   return e == cudaSuccess ? FMS_OK : e == cudaErrorNotSupported ? FMS_ERR_UNSUPPORTED : (int)e;
 }
 
 }  // namespace glu
 
-int read_ffn_device_error(int reset) { return gemm::read_error(reset); }
+int read_ffn_device_error(int reset) {
+  const int a = read_ffn_f16_error(reset), b = read_ffn_bf16_error(reset);
+  return a != 0 ? a : b;
+}
 
 }  // namespace fms
 
@@ -453,7 +53,8 @@ int fms_gated_ffn_fwd(int dtype, const void* x, const void* w_gate, const void* 
     const cudaError_t e = cudaMemsetAsync(h, 0, (size_t)rows * hidden * 2, (cudaStream_t)stream);
     return e == cudaSuccess ? FMS_OK : (int)e;
   }
-  if (!workspace || ws_bytes < fms_gated_ffn_workspace_size(rows, dim, hidden, 0)) return FMS_ERR_WORKSPACE;
+  const size_t need = fms_gated_ffn_workspace_size(rows, dim, hidden, 0);
+  if (need && (!workspace || ws_bytes < need)) return FMS_ERR_WORKSPACE;
   return glu::launch(dtype, act,
                      {x, w_gate, w_up, nullptr, rows, dim, hidden, h, nullptr, nullptr, nullptr, (char*)workspace}, false,
                      (cudaStream_t)stream);

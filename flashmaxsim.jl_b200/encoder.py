@@ -27,15 +27,41 @@ _FLOAT = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def _run(name, dev, *args):
-    if torch.cuda.current_device() == dev.index:
-        _lib.call(name, *args, _lib.stream_of(dev))
+    # one short call: the raw stream, no device switch where none is needed
+    fn = getattr(_lib.lib(), name)
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(dev):
-            _lib.call(name, *args, _lib.stream_of(dev))
+            status = fn(*args, _raw_stream(index))
+    if status != 0:
+        _lib.check(status, name)
 
 
-def _workspace(nbytes, dev):
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+def _raw_stream(index):
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _same_device(*ts):
+    """The one CUDA device of the tensors (None among them is left out)."""
+    index = -2
+    for t in ts:
+        if t is not None:
+            i = t.get_device()
+            if index == -2:
+                index = i
+            if i < 0 or i != index:
+                return _device_of(*ts)  # raises with its reason
+    return next(t for t in ts if t is not None).device
+
+
+def _workspace(nbytes, like):
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 # --------------------------------------------------------------------------- gated feed-forward
@@ -58,12 +84,12 @@ def _ffn_forward(x, w_gate, w_up, act):
     dim, hidden = x.shape[-1], w_gate.shape[0]
     x, w_gate, w_up = x.contiguous(), w_gate.contiguous(), w_up.contiguous()
     dev = x.device
-    h = torch.empty((*x.shape[:-1], hidden), dtype=x.dtype, device=dev)
+    h = x.new_empty((*x.shape[:-1], hidden))
     rows = h.numel() // hidden if hidden else 0
     nb = _lib.lib().fms_gated_ffn_workspace_size(rows, dim, hidden, 0)
-    ws = _workspace(nb, dev)
-    _run("fms_gated_ffn_fwd", dev, _lib.DTYPE_CODE[x.dtype], _lib.ptr(x), _lib.ptr(w_gate),
-         _lib.ptr(w_up), rows, dim, hidden, act, _lib.ptr(h), _lib.ptr(ws), nb)
+    ws = _workspace(nb, x)
+    _run("fms_gated_ffn_fwd", dev, _lib.DTYPE_CODE[x.dtype], _p(x), _p(w_gate),
+         _p(w_up), rows, dim, hidden, act, _p(h), _p(ws), nb)
     return h
 
 
@@ -76,10 +102,10 @@ def _ffn_pullback(dh, x, w_gate, w_up, act, wanted):
     if rows == 0 or hidden == 0:
         return [g if g is None else g.zero_() for g in grads]
     nb = _lib.lib().fms_gated_ffn_workspace_size(rows, dim, hidden, 1)
-    ws = _workspace(nb, dev)
-    _run("fms_gated_ffn_bwd", dev, _lib.DTYPE_CODE[x.dtype], _lib.ptr(x), _lib.ptr(w_gate),
-         _lib.ptr(w_up), _lib.ptr(dh), rows, dim, hidden, act, *map(_lib.ptr, grads),
-         _lib.ptr(ws), nb)
+    ws = _workspace(nb, x)
+    _run("fms_gated_ffn_bwd", dev, _lib.DTYPE_CODE[x.dtype], _p(x), _p(w_gate),
+         _p(w_up), _p(dh), rows, dim, hidden, act, *map(_p, grads),
+         _p(ws), nb)
     return grads
 
 
@@ -102,7 +128,7 @@ def gated_ffn(x, w_gate, w_up, act="silu"):
         raise ArgumentError(f"gated_ffn takes float16 or bfloat16 features, got {x.dtype}")
     if w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
         raise ArgumentError("gated_ffn: features and weights must share an eltype")
-    _device_of(x, w_gate, w_up)
+    _same_device(x, w_gate, w_up)
     if needs_grad(x, w_gate, w_up):
         return _GatedFFN.apply(x, w_gate, w_up, ACTIVATIONS[act])
     return _ffn_forward(x, w_gate, w_up, ACTIVATIONS[act])
@@ -114,11 +140,11 @@ def _norm_forward(x, h, w_post, b_post, w_pre, b_pre, gate, groups, scale, kind,
     dev, dim = x.device, x.shape[-1]
     rows = x.numel() // dim
     z, y = torch.empty_like(x), torch.empty_like(x)
-    stats = torch.empty((4, rows), dtype=torch.float32, device=dev) if want_stats else None
+    stats = x.new_empty((4, rows), dtype=torch.float32) if want_stats else None
     _run("fms_norm_residual_fwd", dev, _lib.DTYPE_CODE[x.dtype], _lib.DTYPE_CODE[w_post.dtype],
-         kind, _lib.ptr(x), _lib.ptr(h), _lib.ptr(w_post), _lib.ptr(b_post), _lib.ptr(w_pre),
-         _lib.ptr(b_pre), _lib.ptr(gate), groups, rows, dim, eps, scale, _lib.ptr(z), _lib.ptr(y),
-         _lib.ptr(stats))
+         kind, _p(x), _p(h), _p(w_post), _p(b_post), _p(w_pre),
+         _p(b_pre), _p(gate), groups, rows, dim, eps, scale, _p(z), _p(y),
+         _p(stats))
     return z, y, stats
 
 
@@ -145,12 +171,12 @@ class _NormResidual(torch.autograd.Function):
         dv = [torch.empty_like(t) if t is not None and need else None for t, need in
               zip((w_post, b_post, w_pre, b_pre, gate), ctx.needs_input_grad[2:7])]
         nb = _lib.lib().fms_norm_residual_bwd_workspace_size(rows, groups, dim)
-        ws = _workspace(nb, dev)
+        ws = _workspace(nb, x)
         _run("fms_norm_residual_bwd", dev, _lib.DTYPE_CODE[x.dtype],
-             _lib.DTYPE_CODE[w_post.dtype], kind, _lib.ptr(x), _lib.ptr(h), _lib.ptr(w_post),
-             _lib.ptr(b_post), _lib.ptr(w_pre), _lib.ptr(gate), groups, rows, dim, scale,
-             _lib.ptr(stats), _lib.ptr(dz), _lib.ptr(dy), _lib.ptr(dx), _lib.ptr(dh),
-             *map(_lib.ptr, dv), _lib.ptr(ws), nb)
+             _lib.DTYPE_CODE[w_post.dtype], kind, _p(x), _p(h), _p(w_post),
+             _p(b_post), _p(w_pre), _p(gate), groups, rows, dim, scale,
+             _p(stats), _p(dz), _p(dy), _p(dx), _p(dh),
+             *map(_p, dv), _p(ws), nb)
         return (dx, dh, *dv, None, None, None, None)
 
 
@@ -192,7 +218,7 @@ def norm_residual(x, h, w_post, w_pre, *, gate=None, b_post=None, b_pre=None, sc
         groups = x.shape[0]
     if not eps >= 0:
         raise ArgumentError("norm_residual: eps must be >= 0")
-    _device_of(x, h, *vectors)
+    _same_device(x, h, *vectors)
     args = [None if t is None else t.contiguous() for t in (x, h, w_post, b_post, w_pre, b_pre, gate)]
     if needs_grad(x, h, *vectors):
         return _NormResidual.apply(*args, groups, float(scale), NORMS[kind], float(eps))
@@ -241,14 +267,14 @@ def int8_linear(x, w: Int8Index, bias=None, out_dtype=None):
         if bias.dtype != out_dtype:
             raise ArgumentError("int8_linear: bias must have the output's eltype")
         bias = bias.contiguous()
-    dev = _device_of(x, xs, codes, scales, bias)
+    dev = _same_device(x, xs, codes, scales, bias)
     x, codes, scales = x.contiguous(), codes.contiguous(), scales.contiguous()
     xs = None if xs is None else xs.contiguous()
-    y = torch.empty((*x.shape[:-1], out), dtype=out_dtype, device=dev)
+    y = x.new_empty((*x.shape[:-1], out), dtype=out_dtype)
     rows = x.numel() // dim
     nb = _lib.lib().fms_int8_linear_workspace_size(xt, rows, dim, out)
-    ws = _workspace(nb, dev)
-    _run("fms_int8_linear_fwd", dev, xt, _lib.ptr(x), _lib.ptr(xs), _lib.ptr(codes),
-         _lib.ptr(scales), _lib.ptr(bias), rows, dim, out, _lib.DTYPE_CODE[out_dtype], _lib.ptr(y),
-         _lib.ptr(ws), nb)
+    ws = _workspace(nb, x)
+    _run("fms_int8_linear_fwd", dev, xt, _p(x), _p(xs), _p(codes),
+         _p(scales), _p(bias), rows, dim, out, _lib.DTYPE_CODE[out_dtype], _p(y),
+         _p(ws), nb)
     return y

@@ -14,6 +14,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .encoder import _run
 from .errors import ArgumentError, DimensionMismatch
 
 BLOCK = 256
@@ -108,12 +109,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
         _same_device(dev, [grad_scale])
     torch.autograd.graph.increment_version(params + m + v + (copies or []))
     args = (8 if eight else 32, n, table.ctypes.data, int(step), float(lr), float(b1), float(b2),
-            float(eps), float(weight_decay), int(seed) & 0xFFFFFFFF, _lib.ptr(grad_scale))
-    if torch.cuda.current_device() == dev.index:
-        _lib.call("fms_adamw_step", *args, _lib.stream_of(dev))
-    else:
-        with torch.cuda.device(dev):
-            _lib.call("fms_adamw_step", *args, _lib.stream_of(dev))
+            float(eps), float(weight_decay), int(seed) & 0xFFFFFFFF, None if grad_scale is None else grad_scale.data_ptr())
+    _run("fms_adamw_step", dev, *args)
 
 
 def moments8(p):
