@@ -18,20 +18,30 @@ from .encoder import _run
 from .errors import ArgumentError, DimensionMismatch
 
 BLOCK = 256
-_FLOAT = (torch.float32, torch.float16, torch.bfloat16)
+_FLOAT = {torch.float32, torch.float16, torch.bfloat16}
+_HALF = {torch.float16, torch.bfloat16}
 _RECORD = np.dtype([("p", "u8"), ("g", "u8"), ("copy", "u8"), ("m", "u8"), ("v", "u8"),
                     ("ms", "u8"), ("vs", "u8"), ("n", "i8"), ("pt", "i4"), ("gt", "i4"),
                     ("ct", "i4"), ("reserved", "i4")])
 
 
-def _same_device(dev, *lists):
-    i = dev.index
-    for ts in lists:
-        for t in ts:
-            if t.get_device() != i:
-                raise ArgumentError("adamw_step: all tensors must live on one CUDA device")
-            if not t.is_contiguous():
-                raise ArgumentError("adamw_step: tensors are updated in place and must be contiguous")
+_get_device = torch.Tensor.get_device
+_is_contiguous = torch.Tensor.is_contiguous
+_numel = torch.Tensor.numel
+_data_ptr = torch.Tensor.data_ptr
+
+
+def _checked(dev, ts):
+    # a model has hundreds of tensors, and this runs every step: whole-list calls
+    if set(map(_get_device, ts)) - {dev.index}:
+        raise ArgumentError("adamw_step: all tensors must live on one CUDA device")
+    if not all(map(_is_contiguous, ts)):
+        raise ArgumentError("adamw_step: tensors are updated in place and must be contiguous")
+    return list(map(_data_ptr, ts))
+
+
+def _dtypes(ts):
+    return [t.dtype for t in ts]
 
 
 @torch.no_grad()
@@ -64,50 +74,50 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
     if dev.type != "cuda":
         raise ArgumentError("adamw_step runs on CUDA tensors only")
     eight = isinstance(exp_avgs[0], (tuple, list))
+    states = exp_avgs + exp_avg_sqs
     if eight:
-        if not all(isinstance(s, (tuple, list)) and len(s) == 2 for s in exp_avgs + exp_avg_sqs):
+        if not all(isinstance(s, (tuple, list)) and len(s) == 2 for s in states):
             raise ArgumentError("adamw_step: moments must all be tensors or all (codes, scales)")
-        ms, vs = [s[1] for s in exp_avgs], [s[1] for s in exp_avg_sqs]
-        m, v = [s[0] for s in exp_avgs], [s[0] for s in exp_avg_sqs]
-        _same_device(dev, ms, vs)
-        if any(s.dtype != torch.float32 for s in ms + vs):
+        scales, states = [s[1] for s in states], [s[0] for s in states]
+        if set(_dtypes(scales)) != {torch.float32}:
             raise ArgumentError("adamw_step: scales of 8-bit moments must be float32")
-    else:
-        m, v = exp_avgs, exp_avg_sqs
-        if not all(isinstance(s, torch.Tensor) for s in m + v):
-            raise ArgumentError("adamw_step: moments must all be tensors or all (codes, scales)")
-    _same_device(dev, params, grads, m, v, copies or ())
+    elif not all(isinstance(s, torch.Tensor) for s in states):
+        raise ArgumentError("adamw_step: moments must all be tensors or all (codes, scales)")
     want = torch.float8_e4m3fn if eight else torch.float32
-    if any(s.dtype != want for s in m + v):
+    if set(_dtypes(states)) != {want}:
         raise ArgumentError(f"adamw_step: moments must hold {want}")
-    if any(t.dtype not in _FLOAT for t in params + grads):
+    pt, gt = _dtypes(params), _dtypes(grads)
+    if not set(pt + gt) <= _FLOAT:
         raise ArgumentError("adamw_step: parameters and gradients must be float32, float16 or bfloat16")
-    if copies is not None and any(t.dtype not in (torch.float16, torch.bfloat16) for t in copies):
+    ct = None if copies is None else _dtypes(copies)
+    if copies is not None and not set(ct) <= _HALF:
         raise ArgumentError("adamw_step: copies must be float16 or bfloat16")
     table = np.zeros(n, _RECORD)
-    sizes = [t.numel() for t in params]
-    for ts in (grads, m, v, copies):
-        if ts is not None and [t.numel() for t in ts] != sizes:
-            raise DimensionMismatch("adamw_step: gradients, moments and copies must have their parameter's size")
+    sizes = list(map(_numel, params))
+    if list(map(_numel, grads)) != sizes or list(map(_numel, states)) != sizes + sizes or \
+            (copies is not None and list(map(_numel, copies)) != sizes):
+        raise DimensionMismatch("adamw_step: gradients, moments and copies must have their parameter's size")
     code = _lib.DTYPE_CODE
     table["n"] = sizes
-    for k, ts in (("p", params), ("g", grads), ("copy", copies), ("m", m), ("v", v)):
-        if ts is not None:
-            table[k] = [t.data_ptr() for t in ts]
-    table["pt"] = [code[t.dtype] for t in params]
-    table["gt"] = [code[t.dtype] for t in grads]
+    table["p"], table["g"] = _checked(dev, params), _checked(dev, grads)
+    at = _checked(dev, states)
+    table["m"], table["v"] = at[:n], at[n:]
+    table["pt"] = [code[t] for t in pt]
+    table["gt"] = [code[t] for t in gt]
     if copies is not None:
-        table["ct"] = [code[t.dtype] for t in copies]
+        table["copy"] = _checked(dev, copies)
+        table["ct"] = [code[t] for t in ct]
     if eight:
         blocks = [-(-s // BLOCK) for s in sizes]
-        if [s.numel() for s in ms] != blocks or [s.numel() for s in vs] != blocks:
+        if list(map(_numel, scales)) != blocks + blocks:
             raise DimensionMismatch("adamw_step: 8-bit moments need one scale per 256 values")
-        table["ms"], table["vs"] = [s.data_ptr() for s in ms], [s.data_ptr() for s in vs]
+        at = _checked(dev, scales)
+        table["ms"], table["vs"] = at[:n], at[n:]
     if grad_scale is not None:
         if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
             raise ArgumentError("adamw_step: grad_scale must be a float32 tensor of one value")
-        _same_device(dev, [grad_scale])
-    torch.autograd.graph.increment_version(params + m + v + (copies or []))
+        _checked(dev, [grad_scale])
+    torch.autograd.graph.increment_version(params + states + (copies or []))
     args = (8 if eight else 32, n, table.ctypes.data, int(step), float(lr), float(b1), float(b2),
             float(eps), float(weight_decay), int(seed) & 0xFFFFFFFF, None if grad_scale is None else grad_scale.data_ptr())
     _run("fms_adamw_step", dev, *args)
