@@ -526,7 +526,7 @@ struct Shape {
   int cg, bn;
   double step;
 };
-constexpr Shape SHAPES[] = {{2, 256, 546.0}, {2, 128, 410.0}, {1, 64, 410.0}};
+constexpr Shape SHAPES[] = {{2, 256, 546.0}, {2, 128, 410.0}, {1, 64, 400.0}};
 inline int pick_shape(int64_t rows, int64_t cols, int kb, int sms) {
   int best = 0;
   double cost = 1e300;

@@ -978,9 +978,16 @@ bool make_map(CUtensorMap* m, int dtype, const void* base, int64_t inner, int64_
                                 : dtype == FMS_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                 : dtype == FMS_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  return enc(m, t, 2, const_cast<void*>(base), gdim, gstride, tile, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  auto encode = [&] {
+    return enc(m, t, 2, const_cast<void*>(base), gdim, gstride, tile, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+           CUDA_SUCCESS;
+  };
+  if (encode()) return true;
+  // A thread that has called nothing of the runtime yet (autograd's, on memory from a
+  // cache) has no context: naming its device binds one.
+  int d;
+  return cudaGetDevice(&d) == cudaSuccess && cudaSetDevice(d) == cudaSuccess && encode();
 }
 }  // namespace gemm
 

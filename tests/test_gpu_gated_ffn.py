@@ -218,6 +218,30 @@ def test_another_stream(fms):
     assert all(torch.equal(got[k], ref[k]) for k in ref)
 
 
+def test_a_thread_without_a_context(fms):
+    """A new host thread, memory from torch's cache: the call is the thread's first of CUDA."""
+    import threading
+    x, wg, wu, _ = make(700, 128, 192, torch.bfloat16, 16)
+    ref = fms.gated_ffn(x, wg, wu)
+    spare = [torch.empty_like(ref), torch.empty(1 << 20, dtype=torch.uint8, device="cuda")]  # noqa: F841
+    torch.cuda.synchronize()
+    del spare
+    got = []
+
+    def work():
+        try:
+            got.append(fms.gated_ffn(x, wg, wu))
+        except Exception as e:  # noqa: BLE001
+            got.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert isinstance(got[0], torch.Tensor), got[0]
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], ref)
+
+
 def test_in_a_cuda_graph(fms):
     x, wg, wu, _ = make(65, 128, 192, torch.bfloat16, 14)
     fms.gated_ffn(x, wg, wu)
