@@ -177,10 +177,12 @@ struct StoreEpi {
   }
 };
 
-// Sum of the parts of a split product, in order.
+// Sum of the parts of a split product, in order; each part holds one or two matrices of
+// `each` values.
 template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int64_t each, T* o0, T* o1) {
-  const int64_t n = 2 * each;
+__global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int64_t each, int outputs, T* o0,
+                                                   T* o1) {
+  const int64_t n = outputs * each;
   if (each % 4 == 0 && ((reinterpret_cast<uintptr_t>(o0) | reinterpret_cast<uintptr_t>(o1)) & 7) == 0) {
     for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
       T* o = i < each ? o0 : o1;
@@ -229,24 +231,27 @@ struct Args {
 static int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 static int64_t tiles(int64_t n, int64_t t) { return (n + t - 1) / t; }
 
-// Parts of the sum over rows for the weights' gradients: enough to give every pair of
-// SMs a tile of about the same length, at least 16 blocks of 64 rows each.
-static int weight_splits(int64_t rows, int dim, int hidden) {
-  const int64_t t = 2 * tiles(hidden, 256) * tiles(dim, 256), pairs = device_sm_count() / 2, kb = tiles(rows, 64);
-  int64_t best = 1;
+// Parts of a sum of kb blocks of 64 for `t` tiles of 256 x 256, whose parts hold `values`
+// float32 each: what gives the shortest time by a pair of SMs doing a block in 0.35 us and
+// starting and ending a tile in 8 blocks' time, and the parts being written and read at 5
+// TB/s in a launch of 2 us more (measured: 4096 x 100 -> 768 in 25 us whole, x us in parts).
+static int parts_of(int64_t t, int kb, int64_t values) {
+  const int64_t pairs = device_sm_count() / 2;
+  int best = 1;
   double cost = 1e30;
-  for (int64_t s = 1; s <= 16 && (s == 1 || kb / s >= 16); ++s) {
-    const double c = (double)tiles(t * s, pairs) * ((double)kb / s + 8.0);  // + a tile's start and end
+  for (int s = 1; s <= 16 && (s == 1 || kb / s >= 4); ++s) {
+    const double c = (double)tiles(t * s, pairs) * ((double)kb / s + 8.0) * 0.35 +
+                     (s > 1 ? 2.0 + 8e-6 * (double)s * (double)values / 5.0 : 0.0);
     if (c < cost * 0.97) cost = c, best = s;
   }
-  return (int)best;
+  return best;
 }
 
 constexpr int FEW = 8;  // rows of the CUDA-core kernel
 
 struct Space {
   size_t x, wg, wu, dh, dg, du, part, total;
-  int ldd, ldh, splits;
+  int ldd, ldh, splits, splits_x;  // parts of the weights' and of the input's gradients
 };
 // Offsets of the workspace.  The padded copies have their place whenever the width
 // asks for them or a pointer might (the size is known without the pointers).
@@ -268,8 +273,11 @@ static Space space(int64_t rows, int dim, int hidden, bool bwd) {
     s.dh = take((size_t)rows * s.ldh * 2);
     s.dg = take((size_t)rows * s.ldh * 2);
     s.du = take((size_t)rows * s.ldh * 2);
-    s.splits = weight_splits(rows, dim, hidden);
-    if (s.splits > 1) s.part = take((size_t)s.splits * 2 * hidden * dim * 4);
+    s.splits = parts_of(2 * tiles(hidden, 256) * tiles(dim, 256), (int)tiles(rows, 64), 2 * (int64_t)hidden * dim);
+    s.splits_x = parts_of(tiles(rows, 256) * tiles(dim, 256), 2 * (int)tiles(hidden, 64), rows * dim);
+    const size_t w = s.splits > 1 ? (size_t)s.splits * 2 * hidden * dim * 4 : 0;
+    const size_t x = s.splits_x > 1 ? (size_t)s.splits_x * rows * dim * 4 : 0;
+    s.part = take(w > x ? w : x);  // one after the other
   }
   s.total = at;
   return s;
@@ -409,11 +417,19 @@ static cudaError_t hidden_any(int dtype, const void* x, const void* wg, const vo
   }
 }
 
+template <typename T>
+static cudaError_t join(const float* part, int splits, int64_t each, int outputs, T* o0, T* o1, cudaStream_t s) {
+  int64_t blocks = tiles(outputs * each, 256 * 4);
+  if (blocks > device_sm_count() * 8) blocks = device_sm_count() * 8;
+  join_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(part, splits, each, outputs, o0, o1);
+  return cudaGetLastError();
+}
+
 // dx = dg Wg + du Wu: the weights as they lie are the second operand with its rows
 // along the sum.
 template <typename T>
 static cudaError_t input_gradient(int dtype, const T* dg, const T* du, const void* wg, const void* wu, int ldd, int ldh,
-                                  const Args& p, cudaStream_t s) {
+                                  int splits, float* part, const Args& p, cudaStream_t s) {
   CUtensorMap a0, a1, b0, b1;
   if (!gemm::make_map(&a0, dtype, dg, p.hidden, p.rows, (int64_t)ldh * 2, 128) ||
       !gemm::make_map(&a1, dtype, du, p.hidden, p.rows, (int64_t)ldh * 2, 128) ||
@@ -423,7 +439,7 @@ static cudaError_t input_gradient(int dtype, const T* dg, const T* du, const voi
   gemm::Work w{};
   w.mt = (int)tiles(p.rows, 256);
   w.nt = (int)tiles(p.dim, 256);
-  w.splits = 1;
+  w.splits = splits;
   w.kb0 = (int)tiles(p.hidden, 64);
   w.kb = 2 * w.kb0;
   w.idesc = gemm::idesc_f16(dtype, 256, 256, false, true);
@@ -431,9 +447,14 @@ static cudaError_t input_gradient(int dtype, const T* dg, const T* du, const voi
   e.o0 = (T*)p.dx;
   e.rows = p.rows;
   e.cols = p.dim;
-  e.mapped = p.dim % 8 == 0 && aligned(p.dx, 16) && gemm::make_map(&e.m0, dtype, p.dx, p.dim, p.rows, (int64_t)p.dim * 2, 32);
-  return gemm::launch<gemm::OP_SUM, 2, 256, false, true, false, StoreEpi<T, false>>(a0, a1, b0, b1, w, e,
-                                                                                    device_sm_count(), s);
+  e.part = splits > 1 ? part : nullptr;
+  e.wide = p.dim % 4 == 0;
+  e.mapped = !e.part && p.dim % 8 == 0 && aligned(p.dx, 16) &&
+             gemm::make_map(&e.m0, dtype, p.dx, p.dim, p.rows, (int64_t)p.dim * 2, 32);
+  const cudaError_t err = gemm::launch<gemm::OP_SUM, 2, 256, false, true, false, StoreEpi<T, false>>(
+      a0, a1, b0, b1, w, e, device_sm_count(), s);
+  if (err != cudaSuccess || splits == 1) return err;
+  return join<T>(part, splits, p.rows * p.dim, 1, (T*)p.dx, nullptr, s);
 }
 
 // dWg = dg^T x over dWu = du^T x: both operands have their rows along the sum.
@@ -466,11 +487,7 @@ static cudaError_t weight_gradients(int dtype, const T* dg, const T* du, const v
   const cudaError_t err = gemm::launch<gemm::OP_STACK_A, 2, 256, true, true, false, StoreEpi<T, true>>(
       a0, a1, b, b, w, e, device_sm_count(), s);
   if (err != cudaSuccess || splits == 1) return err;
-  const int64_t each = (int64_t)p.hidden * p.dim;
-  int64_t blocks = tiles(2 * each, 256 * 4);
-  if (blocks > device_sm_count() * 8) blocks = device_sm_count() * 8;
-  join_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(part, splits, each, (T*)p.dwg, (T*)p.dwu);
-  return cudaGetLastError();
+  return join<T>(part, splits, (int64_t)p.hidden * p.dim, 2, (T*)p.dwg, (T*)p.dwu, s);
 }
 
 template <typename T, int ACT>
@@ -484,7 +501,7 @@ static cudaError_t run(int dtype, const Args& p, bool bwd, cudaStream_t s) {
   const void* dh = pitched(p.dh, p.rows, p.hidden, L.ldh, 32, p.ws + L.dh, s);
   T *dg = (T*)(p.ws + L.dg), *du = (T*)(p.ws + L.du);
   cudaError_t e = hidden_any<T, ACT, true>(dtype, x, wg, wu, L.ldd, dh, L.ldh, p, dg, du, L.ldh, s);
-  if (e == cudaSuccess && p.dx) e = input_gradient<T>(dtype, dg, du, wg, wu, L.ldd, L.ldh, p, s);
+  if (e == cudaSuccess && p.dx) e = input_gradient<T>(dtype, dg, du, wg, wu, L.ldd, L.ldh, L.splits_x, (float*)(p.ws + L.part), p, s);
   if (e == cudaSuccess && (p.dwg || p.dwu))
     e = weight_gradients<T>(dtype, dg, du, x, L.ldd, L.ldh, L.splits, (float*)(p.ws + L.part), p, s);
   return e;
