@@ -402,6 +402,7 @@ __global__ void __launch_bounds__(1024) gather_kernel(Params p, float* out) {
       for (int64_t g = first; g < p.groups; g += step) {
         float s1 = 0.f, s0 = 0.f;
         const int64_t k1 = p.blocks ? block_of(p, (g + 1) * p.per - 1) : -1;
+#pragma unroll 4
         for (int64_t k = p.blocks ? block_of(p, g * p.per) : 0; k <= k1; ++k) {
           s1 += S[(k + g) * p.dim];
           if (BIAS) s0 += S[nS + (k + g) * p.dim];
@@ -413,11 +414,13 @@ __global__ void __launch_bounds__(1024) gather_kernel(Params p, float* out) {
              vec1(p.w_post, p.vdt, c, 1.f) * s1 + vec1(p.b_post, p.vdt, c, 0.f) * s0);
       }
     } else {
+#pragma unroll 4
       for (int64_t k = first; k < p.blocks; k += step) {
         w += S[k * p.dim];
         if (BIAS) b += S[nS + k * p.dim];
       }
     }
+#pragma unroll 4
     for (int64_t k = first; k < p.blocks; k += step) {
       t1 += R[k * p.dim];
       if (BIAS) t0 += R[nT + k * p.dim];
@@ -438,6 +441,7 @@ __global__ void __launch_bounds__(128) finish_kernel(Params p, const float* in, 
   const int c = blockIdx.x * 128 + threadIdx.x;
   if (c >= p.dim) return;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 16
   for (int i = 0; i < parts; ++i)
 #pragma unroll
     for (int k = 0; k < 4; ++k) s[k] += in[((int64_t)i * 4 + k) * p.dim + c];
