@@ -490,20 +490,29 @@ __device__ __forceinline__ void out_store(const unsigned char* out, const CUtens
 template <int SIZE>
 __device__ __forceinline__ void out_rows(const unsigned char* out, void* p, int64_t ld, int rows, int cols, int lane) {
   __syncwarp();
-  char* q = static_cast<char*>(p);
   const bool words = SIZE == 4 || (ld % 2 == 0 && (reinterpret_cast<uintptr_t>(p) & 3) == 0);
   const int c = SIZE == 4 ? lane : 2 * lane;  // of the lane's word
-  for (int r = 0; r < min(rows, 32); ++r) {
-    const uint32_t w =
-        *reinterpret_cast<const uint32_t*>(out + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-    char* at = q + (r * ld + c) * SIZE;
-    if constexpr (SIZE == 4) {
-      if (c < cols) *reinterpret_cast<uint32_t*>(at) = w;
-    } else if (words && c + 1 < cols) {
-      *reinterpret_cast<uint32_t*>(at) = w;
-    } else {
-      if (c < cols) *reinterpret_cast<uint16_t*>(at) = (uint16_t)w;
-      if (c + 1 < cols) *reinterpret_cast<uint16_t*>(at + 2) = (uint16_t)(w >> 16);
+  char* at = static_cast<char*>(p) + (int64_t)c * SIZE;
+  const int64_t step = ld * SIZE;
+  const unsigned char* mine = out + (lane & 3) * 4;
+  rows = min(rows, 32);
+  if (SIZE == 4 || (words && cols == 64)) {  // a word a row
+    if (c < cols) {
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r, at += step)
+        *reinterpret_cast<uint32_t*>(at) =
+            *reinterpret_cast<const uint32_t*>(mine + r * 128 + (((lane >> 2) ^ (r & 7)) << 4));
+    }
+  } else {
+#pragma unroll 4  // (words put together from two lanes for odd rows were slower: 93 us against 73)
+    for (int r = 0; r < rows; ++r, at += step) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(mine + r * 128 + (((lane >> 2) ^ (r & 7)) << 4));
+      if (words && c + 1 < cols) {
+        *reinterpret_cast<uint32_t*>(at) = w;
+      } else {
+        if (c < cols) *reinterpret_cast<uint16_t*>(at) = (uint16_t)w;
+        if (c + 1 < cols) *reinterpret_cast<uint16_t*>(at + 2) = (uint16_t)(w >> 16);
+      }
     }
   }
   __syncwarp();

@@ -118,7 +118,7 @@ struct StoreEpi {
     float* part;
     int64_t rows, pad;
     int cols;
-    int wide;            // rows of `part` start on 16 bytes
+    int ldp;             // elements between the rows of `part`, a multiple of 4
     int mapped;
   };
   template <int BN>
@@ -149,8 +149,8 @@ struct StoreEpi {
       const int n = row < p.rows ? p.cols - col : 0;
       if (p.part) {
         if (n <= 0) continue;
-        float* q = p.part + (at + row) * p.cols + col;
-        if (n >= 32 && p.wide) {
+        float* q = p.part + (at + row) * p.ldp + col;
+        if (n >= 32) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             reinterpret_cast<uint4*>(q)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
@@ -178,45 +178,73 @@ struct StoreEpi {
 };
 
 // Sum of the parts of a split product, in order; each part holds one or two matrices of
-// `each` values.
+// rows x ldp values, of which cols count.
 template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int64_t each, int outputs, T* o0,
-                                                   T* o1) {
-  const int64_t n = outputs * each;
-  if (each % 4 == 0 && ((reinterpret_cast<uintptr_t>(o0) | reinterpret_cast<uintptr_t>(o1)) & 7) == 0) {
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
-      T* o = i < each ? o0 : o1;
-      if (!o) continue;
-      float4 s = *reinterpret_cast<const float4*>(part + i);
-#pragma unroll 4
-      for (int k = 1; k < splits; ++k) {
-        const float4 v = *reinterpret_cast<const float4*>(part + k * n + i);
-        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-      }
-      *reinterpret_cast<uint2*>(o + (i < each ? i : i - each)) =
-          make_uint2(gemm::pack2<T>(s.x, s.y), gemm::pack2<T>(s.z, s.w));
-    }
-    return;
-  }
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+__global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int64_t rows, int cols, int ldp,
+                                                   int outputs, T* o0, T* o1) {
+  const int64_t each = rows * ldp, n = outputs * each;
+  const bool wide = cols == ldp && ((reinterpret_cast<uintptr_t>(o0) | reinterpret_cast<uintptr_t>(o1)) & 7) == 0;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
     T* o = i < each ? o0 : o1;
     if (!o) continue;
-    float s = part[i];
-    for (int k = 1; k < splits; ++k) s += part[k * n + i];
-    o[i < each ? i : i - each] = Tr<T>::from(s);
+    float4 s = *reinterpret_cast<const float4*>(part + i);
+#pragma unroll 4
+    for (int k = 1; k < splits; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(part + k * n + i);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    const int64_t at = i < each ? i : i - each;
+    if (wide) {
+      *reinterpret_cast<uint2*>(o + at) = make_uint2(gemm::pack2<T>(s.x, s.y), gemm::pack2<T>(s.z, s.w));
+    } else {
+      const int64_t r = at / ldp;
+      const int c = (int)(at - r * ldp);
+      const float f[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < cols) o[r * cols + c + j] = Tr<T>::from(f[j]);
+    }
   }
 }
 
-// Rows of `dim` elements copied to rows `ld` apart, for operands whose rows do not
-// start where TMA or a vector load asks; a warp per row.  W: one element or two.
-template <typename W>
-__global__ void __launch_bounds__(256) pitch_kernel(const W* src, int64_t rows, int n, W* dst, int ld) {
-  const int lane = threadIdx.x & 31;
-  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
-    const W* a = src + r * n;
-    W* b = dst + r * ld;
-#pragma unroll 4
-    for (int c = lane; c < n; c += 32) b[c] = a[c];
+// Rows of n elements copied to rows ld apart, for operands whose rows do not start where
+// TMA or a vector load asks; a warp per row, one matrix per blockIdx.y.
+struct Pitch {
+  const uint16_t* src;
+  uint16_t* dst;
+  int64_t rows;
+  int n, ld;
+};
+struct Pitches {
+  Pitch m[4];
+  int count;
+  // The operand with rows that start on `align` bytes: as it is, or the place of its copy.
+  const void* add(const void* p, int64_t rows, int n, int ld, int align, void* copy) {
+    const uintptr_t u = reinterpret_cast<uintptr_t>(p);
+    if (n == ld && (u & (align - 1)) == 0) return p;
+    m[count++] = {(const uint16_t*)p, (uint16_t*)copy, rows, n, ld};
+    return copy;
+  }
+};
+// Pairs of elements at a time: a row that starts on an odd element takes each pair from two
+// neighbouring words (copies are written in whole pairs: ld is even, what lies past n in a
+// row is never read as an element).
+static __global__ void __launch_bounds__(256) pitch_kernel(const Pitches p) {
+  const Pitch& j = p.m[blockIdx.y];
+  const int lane = threadIdx.x & 31, words = j.n / 2;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < j.rows; r += (int64_t)gridDim.x * 8) {
+    const uint16_t* a = j.src + r * j.n;
+    uint32_t* b = reinterpret_cast<uint32_t*>(j.dst + r * j.ld);
+    if ((reinterpret_cast<uintptr_t>(a) & 2) == 0) {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(a);
+#pragma unroll 8
+      for (int c = lane; c < words; c += 32) b[c] = w[c];
+    } else {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(a - 1);
+#pragma unroll 8
+      for (int c = lane; c < words; c += 32) b[c] = __funnelshift_r(w[c], w[c + 1], 16);
+    }
+    if (lane == 0 && j.n % 2 != 0) b[words] = a[j.n - 1];  // the last element, alone
   }
 }
 
@@ -275,8 +303,8 @@ static Space space(int64_t rows, int dim, int hidden, bool bwd) {
     s.du = take((size_t)rows * s.ldh * 2);
     s.splits = parts_of(2 * tiles(hidden, 256) * tiles(dim, 256), (int)tiles(rows, 64), 2 * (int64_t)hidden * dim);
     s.splits_x = parts_of(tiles(rows, 256) * tiles(dim, 256), 2 * (int)tiles(hidden, 64), rows * dim);
-    const size_t w = s.splits > 1 ? (size_t)s.splits * 2 * hidden * dim * 4 : 0;
-    const size_t x = s.splits_x > 1 ? (size_t)s.splits_x * rows * dim * 4 : 0;
+    const size_t w = s.splits > 1 ? (size_t)s.splits * 2 * hidden * up(dim, 4) * 4 : 0;
+    const size_t x = s.splits_x > 1 ? (size_t)s.splits_x * rows * up(dim, 4) * 4 : 0;
     s.part = take(w > x ? w : x);  // one after the other
   }
   s.total = at;
@@ -285,17 +313,14 @@ static Space space(int64_t rows, int dim, int hidden, bool bwd) {
 
 static bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-// The operand with rows that start on `align` bytes: as it is, or copied to rows of ld
-// elements.
-static const void* pitched(const void* p, int64_t rows, int dim, int ld, int align, char* copy, cudaStream_t s) {
-  if (dim == ld && aligned(p, align)) return p;
-  int64_t b = tiles(rows, 8);
+static cudaError_t run_pitches(const Pitches& p, cudaStream_t s) {
+  if (p.count == 0) return cudaSuccess;
+  int64_t most = 1;
+  for (int i = 0; i < p.count; ++i) most = p.m[i].rows > most ? p.m[i].rows : most;
+  int64_t b = tiles(most, 8);
   if (b > device_sm_count() * 8) b = device_sm_count() * 8;
-  if (dim % 2 == 0 && aligned(p, 4))
-    pitch_kernel<uint32_t><<<(unsigned)b, 256, 0, s>>>((const uint32_t*)p, rows, dim / 2, (uint32_t*)copy, ld / 2);
-  else
-    pitch_kernel<uint16_t><<<(unsigned)b, 256, 0, s>>>((const uint16_t*)p, rows, dim, (uint16_t*)copy, ld);
-  return copy;
+  pitch_kernel<<<dim3((unsigned)b, (unsigned)p.count), 256, 0, s>>>(p);
+  return cudaGetLastError();
 }
 
 // ------------------------------------------------------------------ a few rows
@@ -418,10 +443,12 @@ static cudaError_t hidden_any(int dtype, const void* x, const void* wg, const vo
 }
 
 template <typename T>
-static cudaError_t join(const float* part, int splits, int64_t each, int outputs, T* o0, T* o1, cudaStream_t s) {
-  int64_t blocks = tiles(outputs * each, 256 * 4);
+static cudaError_t join(const float* part, int splits, int64_t rows, int cols, int outputs, T* o0, T* o1,
+                        cudaStream_t s) {
+  const int ldp = (int)up(cols, 4);
+  int64_t blocks = tiles(outputs * rows * ldp, 256 * 4);
   if (blocks > device_sm_count() * 8) blocks = device_sm_count() * 8;
-  join_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(part, splits, each, outputs, o0, o1);
+  join_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(part, splits, rows, cols, ldp, outputs, o0, o1);
   return cudaGetLastError();
 }
 
@@ -448,13 +475,13 @@ static cudaError_t input_gradient(int dtype, const T* dg, const T* du, const voi
   e.rows = p.rows;
   e.cols = p.dim;
   e.part = splits > 1 ? part : nullptr;
-  e.wide = p.dim % 4 == 0;
+  e.ldp = (int)up(p.dim, 4);
   e.mapped = !e.part && p.dim % 8 == 0 && aligned(p.dx, 16) &&
              gemm::make_map(&e.m0, dtype, p.dx, p.dim, p.rows, (int64_t)p.dim * 2, 32);
   const cudaError_t err = gemm::launch<gemm::OP_SUM, 2, 256, false, true, false, StoreEpi<T, false>>(
       a0, a1, b0, b1, w, e, device_sm_count(), s);
   if (err != cudaSuccess || splits == 1) return err;
-  return join<T>(part, splits, p.rows * p.dim, 1, (T*)p.dx, nullptr, s);
+  return join<T>(part, splits, p.rows, p.dim, 1, (T*)p.dx, nullptr, s);
 }
 
 // dWg = dg^T x over dWu = du^T x: both operands have their rows along the sum.
@@ -480,27 +507,30 @@ static cudaError_t weight_gradients(int dtype, const T* dg, const T* du, const v
   e.rows = p.hidden;
   e.pad = (int64_t)w.mt0 * 256;
   e.cols = p.dim;
-  e.wide = p.dim % 4 == 0;
+  e.ldp = (int)up(p.dim, 4);
   e.mapped = !e.part && p.dim % 8 == 0 && p.dwg && p.dwu && aligned(p.dwg, 16) && aligned(p.dwu, 16) &&
              gemm::make_map(&e.m0, dtype, p.dwg, p.dim, p.hidden, (int64_t)p.dim * 2, 32) &&
              gemm::make_map(&e.m1, dtype, p.dwu, p.dim, p.hidden, (int64_t)p.dim * 2, 32);
   const cudaError_t err = gemm::launch<gemm::OP_STACK_A, 2, 256, true, true, false, StoreEpi<T, true>>(
       a0, a1, b, b, w, e, device_sm_count(), s);
   if (err != cudaSuccess || splits == 1) return err;
-  return join<T>(part, splits, (int64_t)p.hidden * p.dim, 2, (T*)p.dwg, (T*)p.dwu, s);
+  return join<T>(part, splits, p.hidden, p.dim, 2, (T*)p.dwg, (T*)p.dwu, s);
 }
 
 template <typename T, int ACT>
 static cudaError_t run(int dtype, const Args& p, bool bwd, cudaStream_t s) {
   if (!bwd && p.rows <= FEW) return p.rows == 1 ? few_rows<T, ACT, 1>(p, s) : few_rows<T, ACT, FEW>(p, s);
   const Space L = space(p.rows, p.dim, p.hidden, bwd);
-  const void* x = pitched(p.x, p.rows, p.dim, L.ldd, 16, p.ws + L.x, s);
-  const void* wg = pitched(p.wg, p.hidden, p.dim, L.ldd, 16, p.ws + L.wg, s);
-  const void* wu = pitched(p.wu, p.hidden, p.dim, L.ldd, 16, p.ws + L.wu, s);
+  Pitches c{};
+  const void* x = c.add(p.x, p.rows, p.dim, L.ldd, 16, p.ws + L.x);
+  const void* wg = c.add(p.wg, p.hidden, p.dim, L.ldd, 16, p.ws + L.wg);
+  const void* wu = c.add(p.wu, p.hidden, p.dim, L.ldd, 16, p.ws + L.wu);
+  const void* dh = bwd ? c.add(p.dh, p.rows, p.hidden, L.ldh, 32, p.ws + L.dh) : nullptr;
+  cudaError_t e = run_pitches(c, s);
+  if (e != cudaSuccess) return e;
   if (!bwd) return hidden_any<T, ACT, false>(dtype, x, wg, wu, L.ldd, nullptr, 0, p, (T*)p.h, nullptr, p.hidden, s);
-  const void* dh = pitched(p.dh, p.rows, p.hidden, L.ldh, 32, p.ws + L.dh, s);
   T *dg = (T*)(p.ws + L.dg), *du = (T*)(p.ws + L.du);
-  cudaError_t e = hidden_any<T, ACT, true>(dtype, x, wg, wu, L.ldd, dh, L.ldh, p, dg, du, L.ldh, s);
+  e = hidden_any<T, ACT, true>(dtype, x, wg, wu, L.ldd, dh, L.ldh, p, dg, du, L.ldh, s);
   if (e == cudaSuccess && p.dx) e = input_gradient<T>(dtype, dg, du, wg, wu, L.ldd, L.ldh, L.splits_x, (float*)(p.ws + L.part), p, s);
   if (e == cudaSuccess && (p.dwg || p.dwu))
     e = weight_gradients<T>(dtype, dg, du, x, L.ldd, L.ldh, L.splits, (float*)(p.ws + L.part), p, s);
