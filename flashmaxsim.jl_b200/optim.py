@@ -10,7 +10,9 @@ values; the second moment's codes are those of its square root.
 """
 from __future__ import annotations
 
-import numpy as np
+import struct
+from itertools import repeat
+
 import torch
 
 from . import _lib
@@ -20,9 +22,8 @@ from .errors import ArgumentError, DimensionMismatch
 BLOCK = 256
 _FLOAT = {torch.float32, torch.float16, torch.bfloat16}
 _HALF = {torch.float16, torch.bfloat16}
-_RECORD = np.dtype([("p", "u8"), ("g", "u8"), ("copy", "u8"), ("m", "u8"), ("v", "u8"),
-                    ("ms", "u8"), ("vs", "u8"), ("n", "i8"), ("pt", "i4"), ("gt", "i4"),
-                    ("ct", "i4"), ("reserved", "i4")])
+# one fms_adamw_tensor: p, g, copy, m, v, m_scales, v_scales, n, and the codes of three types
+_pack = struct.Struct("=7QqiiiI").pack
 
 
 _get_device = torch.Tensor.get_device
@@ -92,34 +93,30 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
     ct = None if copies is None else _dtypes(copies)
     if copies is not None and not set(ct) <= _HALF:
         raise ArgumentError("adamw_step: copies must be float16 or bfloat16")
-    table = np.zeros(n, _RECORD)
     sizes = list(map(_numel, params))
     if list(map(_numel, grads)) != sizes or list(map(_numel, states)) != sizes + sizes or \
             (copies is not None and list(map(_numel, copies)) != sizes):
         raise DimensionMismatch("adamw_step: gradients, moments and copies must have their parameter's size")
-    code = _lib.DTYPE_CODE
-    table["n"] = sizes
-    table["p"], table["g"] = _checked(dev, params), _checked(dev, grads)
-    at = _checked(dev, states)
-    table["m"], table["v"] = at[:n], at[n:]
-    table["pt"] = [code[t] for t in pt]
-    table["gt"] = [code[t] for t in gt]
-    if copies is not None:
-        table["copy"] = _checked(dev, copies)
-        table["ct"] = [code[t] for t in ct]
+    at = _checked(dev, params + grads + states + (copies or []))
+    p, g, m, v, c = at[:n], at[n:2 * n], at[2 * n:3 * n], at[3 * n:4 * n], at[4 * n:]
+    ms = vs = none = repeat(0)
     if eight:
         blocks = [-(-s // BLOCK) for s in sizes]
         if list(map(_numel, scales)) != blocks + blocks:
             raise DimensionMismatch("adamw_step: 8-bit moments need one scale per 256 values")
         at = _checked(dev, scales)
-        table["ms"], table["vs"] = at[:n], at[n:]
+        ms, vs = at[:n], at[n:]
+    code = _lib.DTYPE_CODE.__getitem__
+    table = b"".join(map(_pack, p, g, c or none, m, v, ms, vs, sizes, map(code, pt), map(code, gt),
+                         none if ct is None else map(code, ct), none))
     if grad_scale is not None:
         if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
             raise ArgumentError("adamw_step: grad_scale must be a float32 tensor of one value")
         _checked(dev, [grad_scale])
     torch.autograd.graph.increment_version(params + states + (copies or []))
-    args = (8 if eight else 32, n, table.ctypes.data, int(step), float(lr), float(b1), float(b2),
-            float(eps), float(weight_decay), int(seed) & 0xFFFFFFFF, None if grad_scale is None else grad_scale.data_ptr())
+    args = (8 if eight else 32, n, table, int(step), float(lr), float(b1), float(b2),
+            float(eps), float(weight_decay), int(seed) & 0xFFFFFFFF,
+            None if grad_scale is None else grad_scale.data_ptr())
     _run("fms_adamw_step", dev, *args)
 
 
