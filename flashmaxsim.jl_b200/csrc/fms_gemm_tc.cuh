@@ -22,6 +22,7 @@
 
 #include "fms_common.cuh"
 #include "fms_internal.h"
+#include "fms_launch.cuh"
 #include "fms_tc_ptx.cuh"
 
 namespace fms {
@@ -265,6 +266,7 @@ kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensor
   __syncthreads();
   if (CG == 2) cluster_sync_all();
   ptx::tc_fence_after();
+  dependency_wait();
   const uint32_t tmem = tmem_s;
   const int64_t tiles = (int64_t)W.mt * W.nt * W.splits;
   const int64_t first = blockIdx.x / CG, stride = gridDim.x / CG;
@@ -564,11 +566,13 @@ cudaError_t launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorM
   c.blockDim = dim3(NTHREADS);
   c.dynamicSmemBytes = smem;
   c.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim = {(unsigned)CG, 1, 1};
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim = {(unsigned)CG, 1, 1};
   c.attrs = at;
-  c.numAttrs = CG == 2 ? 1 : 0;
+  c.numAttrs = CG == 2 ? 2 : 1;
   return cudaLaunchKernelEx(&c, k, a0, a1, b0, b1, w, e);
 }
 

@@ -182,6 +182,7 @@ struct StoreEpi {
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int64_t rows, int cols, int ldp,
                                                    int outputs, T* o0, T* o1) {
+  dependency_wait();
   const int64_t each = rows * ldp, n = outputs * each;
   const bool wide = cols == ldp && ((reinterpret_cast<uintptr_t>(o0) | reinterpret_cast<uintptr_t>(o1)) & 7) == 0;
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
@@ -230,6 +231,7 @@ struct Pitches {
 // neighbouring words (copies are written in whole pairs: ld is even, what lies past n in a
 // row is never read as an element).
 static __global__ void __launch_bounds__(256) pitch_kernel(const Pitches p) {
+  dependency_wait();
   const Pitch& j = p.m[blockIdx.y];
   const int lane = threadIdx.x & 31, words = j.n / 2;
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < j.rows; r += (int64_t)gridDim.x * 8) {
@@ -319,8 +321,7 @@ static cudaError_t run_pitches(const Pitches& p, cudaStream_t s) {
   for (int i = 0; i < p.count; ++i) most = p.m[i].rows > most ? p.m[i].rows : most;
   int64_t b = tiles(most, 8);
   if (b > device_sm_count() * 8) b = device_sm_count() * 8;
-  pitch_kernel<<<dim3((unsigned)b, (unsigned)p.count), 256, 0, s>>>(p);
-  return cudaGetLastError();
+  return launch_after(pitch_kernel, dim3((unsigned)b, (unsigned)p.count), dim3(256), 0, s, p);
 }
 
 // ------------------------------------------------------------------ a few rows
@@ -334,6 +335,7 @@ __global__ void __launch_bounds__(128) few_kernel(const T* x, const T* wg, const
                                                   T* h) {
   const int lane = threadIdx.x & 31;
   const int f = blockIdx.x * 4 + (threadIdx.x >> 5);
+  dependency_wait();
   if (f >= hidden) return;
   float2 g[NR], u[NR];
 #pragma unroll
@@ -425,10 +427,10 @@ static cudaError_t few_rows(const Args& p, cudaStream_t s) {
   const unsigned blocks = (unsigned)tiles(p.hidden, 4);
   const T *x = (const T*)p.x, *wg = (const T*)p.wg, *wu = (const T*)p.wu;
   if (p.dim % 8 == 0 && aligned(x, 16) && aligned(wg, 16) && aligned(wu, 16))
-    few_kernel<T, ACT, NR, true><<<blocks, 128, 0, s>>>(x, wg, wu, (int)p.rows, p.dim, p.hidden, (T*)p.h);
-  else
-    few_kernel<T, ACT, NR, false><<<blocks, 128, 0, s>>>(x, wg, wu, (int)p.rows, p.dim, p.hidden, (T*)p.h);
-  return cudaGetLastError();
+    return launch_after(few_kernel<T, ACT, NR, true>, dim3(blocks), dim3(128), 0, s, x, wg, wu, (int)p.rows, p.dim,
+                        p.hidden, (T*)p.h);
+  return launch_after(few_kernel<T, ACT, NR, false>, dim3(blocks), dim3(128), 0, s, x, wg, wu, (int)p.rows, p.dim, p.hidden,
+                      (T*)p.h);
 }
 
 template <typename T, int ACT, bool BWD>
@@ -448,8 +450,8 @@ static cudaError_t join(const float* part, int splits, int64_t rows, int cols, i
   const int ldp = (int)up(cols, 4);
   int64_t blocks = tiles(outputs * rows * ldp, 256 * 4);
   if (blocks > device_sm_count() * 8) blocks = device_sm_count() * 8;
-  join_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(part, splits, rows, cols, ldp, outputs, o0, o1);
-  return cudaGetLastError();
+  return launch_after(join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, part, splits, rows, cols, ldp, outputs, o0,
+                      o1);
 }
 
 // dx = dg Wg + du Wu: the weights as they lie are the second operand with its rows

@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* x, int64_t rows,
   const int warp = threadIdx.x >> 5, tid = threadIdx.x % TPR;
   const int64_t t = (int64_t)blockIdx.x * (8 / W) + threadIdx.x / TPR;
   const bool real = t < rows;
+  dependency_wait();
   const uint4* xt = reinterpret_cast<const uint4*>(x + t * K);
   uint4 v[NV];
   uint32_t top = 0;  // bits of the largest |x|; as whole numbers a NaN's are above infinity's
@@ -123,6 +124,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) quantize_any_kernel(const T* x, int64_t rows, int K, int8_t* codes, int pitch,
                                                            float* scales) {
   __shared__ uint32_t part[8];
+  dependency_wait();
   for (int64_t t = blockIdx.x; t < rows; t += gridDim.x) {
     const T* xt = x + t * K;
     uint32_t top = 0;
@@ -152,6 +154,7 @@ __global__ void __launch_bounds__(256) few_kernel(const X* x, const float* x_sca
   __shared__ float sx[NTOK];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int pitch = (K + 15) & ~15;
+  dependency_wait();
   for (int t = warp; t < rows; t += 8) {
     unsigned char* ct = codes_s + t * pitch;
     if constexpr (sizeof(X) == 1) {
@@ -284,38 +287,41 @@ static bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(
 
 // Bytes copied to rows `pitch` apart, for codes whose rows do not start on 16 bytes.
 __global__ void __launch_bounds__(256) pitch_kernel(const int8_t* src, int64_t rows, int K, int8_t* dst, int pitch) {
+  dependency_wait();
   const int64_t n = rows * K;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
     dst[i / K * pitch + i % K] = src[i];
 }
-static const int8_t* pitched(const int8_t* p, int64_t rows, int K, int8_t* copy, cudaStream_t s) {
-  if (K % 16 == 0 && aligned(p, 16)) return p;
+static cudaError_t pitched(const int8_t*& p, int64_t rows, int K, int8_t* copy, cudaStream_t s) {
+  if (K % 16 == 0 && aligned(p, 16)) return cudaSuccess;
   int64_t b = (rows * K + 2047) / 2048;
-  if (b > 148 * 16) b = 148 * 16;
-  pitch_kernel<<<(unsigned)b, 256, 0, s>>>(p, rows, K, copy, pitch_of(K));
-  return copy;
+  if (b > device_sm_count() * 16) b = device_sm_count() * 16;
+  const cudaError_t e = launch_after(pitch_kernel, dim3((unsigned)b), dim3(256), 0, s, p, rows, K, copy, pitch_of(K));
+  p = copy;
+  return e;
 }
 
 template <typename T>
-static void quantize(const void* xv, int64_t rows, int K, int8_t* codes, float* scales, cudaStream_t s) {
+static cudaError_t quantize(const void* xv, int64_t rows, int K, int8_t* codes, float* scales, cudaStream_t s) {
   const T* x = (const T*)xv;
   constexpr int N = Vec<T>::N;
   const int pitch = pitch_of(K);
   if (K % N != 0 || !aligned(x, 16) || K > 32 * N * 32) {
-    quantize_any_kernel<T><<<(unsigned)(rows < 148 * 8 ? rows : 148 * 8), 256, 0, s>>>(x, rows, K, codes, pitch, scales);
-    return;
+    const int64_t most = (int64_t)device_sm_count() * 8;
+    return launch_after(quantize_any_kernel<T>, dim3((unsigned)(rows < most ? rows : most)), dim3(256), 0, s, x, rows, K,
+                        codes, pitch, scales);
   }
   auto go = [&](auto kernel, int w) {
-    kernel<<<(unsigned)((rows * w + 7) / 8), 256, 0, s>>>(x, rows, K, codes, pitch, scales);
+    return launch_after(kernel, dim3((unsigned)((rows * w + 7) / 8)), dim3(256), 0, s, x, rows, K, codes, pitch, scales);
   };
   const int nv = (K + 32 * N - 1) / (32 * N);
-  if (nv <= 1) go(quantize_kernel<T, 1, 1>, 1);
-  else if (nv <= 2) go(quantize_kernel<T, 2, 1>, 1);
-  else if (nv <= 3) go(quantize_kernel<T, 3, 1>, 1);
-  else if (nv <= 4) go(quantize_kernel<T, 4, 1>, 1);
-  else if (nv <= 8) go(quantize_kernel<T, 4, 2>, 2);
-  else if (nv <= 16) go(quantize_kernel<T, 4, 4>, 4);
-  else go(quantize_kernel<T, 4, 8>, 8);
+  if (nv <= 1) return go(quantize_kernel<T, 1, 1>, 1);
+  if (nv <= 2) return go(quantize_kernel<T, 2, 1>, 1);
+  if (nv <= 3) return go(quantize_kernel<T, 3, 1>, 1);
+  if (nv <= 4) return go(quantize_kernel<T, 4, 1>, 1);
+  if (nv <= 8) return go(quantize_kernel<T, 4, 2>, 2);
+  if (nv <= 16) return go(quantize_kernel<T, 4, 4>, 4);
+  return go(quantize_kernel<T, 4, 8>, 8);
 }
 
 struct Args {
@@ -352,13 +358,13 @@ static cudaError_t run_few(const Args& p, cudaStream_t s) {
   const X* x = (const X*)p.x;
   const Y* bias = (const Y*)p.bias;
   Y* y = (Y*)p.y;
-  if (p.K % 16 == 0 && aligned(p.wc, 16))
-    few_kernel<X, Y, NTOK, 16><<<blocks, 256, smem, s>>>(x, p.x_scales, p.wc, p.sw, bias, (int)p.rows, p.K, p.C, y);
-  else if (p.K % 4 == 0 && aligned(p.wc, 4))
-    few_kernel<X, Y, NTOK, 4><<<blocks, 256, smem, s>>>(x, p.x_scales, p.wc, p.sw, bias, (int)p.rows, p.K, p.C, y);
-  else
-    few_kernel<X, Y, NTOK, 1><<<blocks, 256, smem, s>>>(x, p.x_scales, p.wc, p.sw, bias, (int)p.rows, p.K, p.C, y);
-  return cudaGetLastError();
+  auto go = [&](auto kernel) {
+    return launch_after(kernel, dim3((unsigned)blocks), dim3(256), smem, s, x, p.x_scales, p.wc, p.sw, bias, (int)p.rows,
+                        p.K, p.C, y);
+  };
+  if (p.K % 16 == 0 && aligned(p.wc, 16)) return go(few_kernel<X, Y, NTOK, 16>);
+  if (p.K % 4 == 0 && aligned(p.wc, 4)) return go(few_kernel<X, Y, NTOK, 4>);
+  return go(few_kernel<X, Y, NTOK, 1>);
 }
 
 template <typename Y, int CG, int BN>
@@ -391,18 +397,21 @@ static cudaError_t run(const Args& p, cudaStream_t s) {
   if (few(p.rows, p.K)) return p.rows == 1 ? run_few<X, Y, 1>(p, s) : run_few<X, Y, FEW>(p, s);
   const Space L = space(sizeof(X) == 1 ? FMS_I8 : FMS_F32, p.rows, p.K, p.C);
   int8_t* codes = (int8_t*)(p.ws + L.codes);
-  const int8_t* xc;
+  const int8_t *xc, *wc = p.wc;
   const float* sx;
+  cudaError_t e = pitched(wc, p.C, p.K, (int8_t*)(p.ws + L.w), s);
+  if (e != cudaSuccess) return e;
   if constexpr (sizeof(X) == 1) {
-    xc = pitched((const int8_t*)p.x, p.rows, p.K, codes, s);
+    xc = (const int8_t*)p.x;
+    e = pitched(xc, p.rows, p.K, codes, s);
     sx = p.x_scales;
   } else {
     float* sc = (float*)(p.ws + L.scales);
-    quantize<X>(p.x, p.rows, p.K, codes, sc, s);
+    e = quantize<X>(p.x, p.rows, p.K, codes, sc, s);
     xc = codes;
     sx = sc;
   }
-  const int8_t* wc = pitched(p.wc, p.C, p.K, (int8_t*)(p.ws + L.w), s);
+  if (e != cudaSuccess) return e;
   switch (gemm::pick_shape(p.rows, p.C, (p.K + 127) / 128, device_sm_count())) {
     case 0: return product<Y, 2, 256>(xc, sx, wc, p, s);
     case 1: return product<Y, 2, 128>(xc, sx, wc, p, s);

@@ -30,6 +30,7 @@
 // row).
 #include "fms_common.cuh"
 #include "fms_internal.h"
+#include "fms_launch.cuh"
 
 #include <type_traits>
 
@@ -187,6 +188,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) forward_kernel(Params p) {
   __shared__ float part[2][MAX_WARPS];
   RowSum<WARP, 1> sum{part};
   const int64_t r = WARP ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  dependency_wait();
   if (WARP && r >= p.rows) return;
   const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, tpr = WARP ? 32 : blockDim.x;
   const int D = p.dim;
@@ -283,6 +285,7 @@ template <typename T, int VEC, int N, bool BIAS>
 __global__ void __launch_bounds__(512) backward_kernel(Params p) {
   __shared__ float part[2][MAX_WARPS * 2];
   RowSum<false, 2> sum{part};
+  dependency_wait();
   const int D = p.dim, tid = threadIdx.x, tpr = blockDim.x;
   const float inv_d = 1.f / D;
   const int64_t r0 = p.rows * blockIdx.x / p.blocks, r1 = p.rows * (blockIdx.x + 1) / p.blocks;
@@ -390,6 +393,7 @@ __global__ void __launch_bounds__(512) backward_kernel(Params p) {
 template <bool BIAS>
 __global__ void __launch_bounds__(1024) gather_kernel(Params p, float* out) {
   __shared__ float acc[4][32][33];
+  dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   const float* S = p.part + c;
@@ -439,6 +443,7 @@ __global__ void __launch_bounds__(1024) gather_kernel(Params p, float* out) {
 
 __global__ void __launch_bounds__(128) finish_kernel(Params p, const float* in, int parts) {
   const int c = blockIdx.x * 128 + threadIdx.x;
+  dependency_wait();
   if (c >= p.dim) return;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 16
@@ -476,10 +481,10 @@ static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 template <typename T, int VEC, int N, bool WARP>
 static void forward(const Params& p, cudaStream_t s) {
   if constexpr (WARP) {
-    forward_kernel<T, VEC, N, true><<<(unsigned)((p.rows + 3) / 4), 128, 0, s>>>(p);
+    launch_after(forward_kernel<T, VEC, N, true>, dim3((unsigned)((p.rows + 3) / 4)), dim3(128), 0, s, p);
   } else {
     const int tpr = (p.dim + 2 * N * 32 - 1) / (2 * N * 32) * 32;
-    forward_kernel<T, VEC, N, false><<<(unsigned)p.rows, tpr, 0, s>>>(p);
+    launch_after(forward_kernel<T, VEC, N, false>, dim3((unsigned)p.rows), dim3(tpr), 0, s, p);
   }
 }
 
@@ -496,7 +501,7 @@ static void run_forward(const Params& p, cudaStream_t s) {
 template <typename T, int VEC, int N, bool BIAS>
 static void backward(const Params& p, cudaStream_t s) {
   const int tpr = (p.dim + 2 * N * 32 - 1) / (2 * N * 32) * 32;
-  backward_kernel<T, VEC, N, BIAS><<<(unsigned)p.blocks, tpr, 0, s>>>(p);
+  launch_after(backward_kernel<T, VEC, N, BIAS>, dim3((unsigned)p.blocks), dim3(tpr), 0, s, p);
 }
 
 template <typename T, int VEC, bool BIAS>
@@ -528,9 +533,8 @@ static void run(const Params& p, bool bwd, cudaStream_t s) {
   const int parts = parts_of(p.groups, p.blocks);
   float* sums = p.part + (4 * p.blocks + 2 * p.groups) * p.dim;
   const dim3 grid((unsigned)((p.dim + 31) / 32), (unsigned)parts);
-  if (bias) gather_kernel<true><<<grid, 1024, 0, s>>>(p, sums);
-  else gather_kernel<false><<<grid, 1024, 0, s>>>(p, sums);
-  finish_kernel<<<(unsigned)((p.dim + 127) / 128), 128, 0, s>>>(p, sums, parts);
+  launch_after(bias ? gather_kernel<true> : gather_kernel<false>, grid, dim3(1024), 0, s, p, sums);
+  launch_after(finish_kernel, dim3((unsigned)((p.dim + 127) / 128)), dim3(128), 0, s, p, (const float*)sums, parts);
 }
 
 static int launch(int dtype, const Params& p, bool bwd, cudaStream_t s) {
