@@ -498,23 +498,23 @@ __device__ __forceinline__ void out_rows(const unsigned char* out, void* p, int6
   const int64_t step = ld * SIZE;
   const unsigned char* mine = out + (lane & 3) * 4;
   rows = min(rows, 32);
-  if (SIZE == 4 || (words && cols == 64)) {  // a word a row
-    if (c < cols) {
+  if (SIZE == 4 || words) {
+    if (c + (SIZE == 4 ? 0 : 1) < cols) {  // a word a row
 #pragma unroll 8
       for (int r = 0; r < rows; ++r, at += step)
         *reinterpret_cast<uint32_t*>(at) =
             *reinterpret_cast<const uint32_t*>(mine + r * 128 + (((lane >> 2) ^ (r & 7)) << 4));
+    } else if (c < cols) {  // the last column, alone
+      for (int r = 0; r < rows; ++r, at += step)
+        *reinterpret_cast<uint16_t*>(at) =
+            *reinterpret_cast<const uint16_t*>(mine + r * 128 + (((lane >> 2) ^ (r & 7)) << 4));
     }
   } else {
 #pragma unroll 4  // (words put together from two lanes for odd rows were slower: 93 us against 73)
     for (int r = 0; r < rows; ++r, at += step) {
       const uint32_t w = *reinterpret_cast<const uint32_t*>(mine + r * 128 + (((lane >> 2) ^ (r & 7)) << 4));
-      if (words && c + 1 < cols) {
-        *reinterpret_cast<uint32_t*>(at) = w;
-      } else {
-        if (c < cols) *reinterpret_cast<uint16_t*>(at) = (uint16_t)w;
-        if (c + 1 < cols) *reinterpret_cast<uint16_t*>(at + 2) = (uint16_t)(w >> 16);
-      }
+      if (c < cols) *reinterpret_cast<uint16_t*>(at) = (uint16_t)w;
+      if (c + 1 < cols) *reinterpret_cast<uint16_t*>(at + 2) = (uint16_t)(w >> 16);
     }
   }
   __syncwarp();

@@ -30,17 +30,13 @@ def _run(name, dev, *args):
     # one short call: the raw stream, no device switch where none is needed
     fn = getattr(_lib.lib(), name)
     index = dev.index
-    if torch.cuda.current_device() == index:
-        status = fn(*args, _raw_stream(index))
+    if torch._C._cuda_getDevice() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            status = fn(*args, _raw_stream(index))
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if status != 0:
         _lib.check(status, name)
-
-
-def _raw_stream(index):
-    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _p(t):
