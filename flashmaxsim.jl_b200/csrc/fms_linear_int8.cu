@@ -119,6 +119,28 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* x, int64_t rows,
   if (tid == 0) scales[t] = s.s;
 }
 
+// Rows of up to 32 NE values that start anywhere: a warp each, a value per lane at a time.
+template <typename T, int NE>
+__global__ void __launch_bounds__(256) quantize_odd_kernel(const T* x, int64_t rows, int K, int8_t* codes, int pitch,
+                                                           float* scales) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  dependency_wait();
+  if (t >= rows) return;
+  const T* xt = x + t * K;
+  T v[NE];
+#pragma unroll
+  for (int i = 0; i < NE; ++i) v[i] = i * 32 + lane < K ? xt[i * 32 + lane] : Tr<T>::from(0.f);
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) top = max(top, abs_bits(Tr<T>::to(v[i])));
+  const Scale s = make_scale(__reduce_max_sync(0xffffffffu, top));
+#pragma unroll
+  for (int i = 0; i < NE; ++i)
+    if (i * 32 + lane < K) codes[t * pitch + i * 32 + lane] = (int8_t)code(Tr<T>::to(v[i]), s);
+  if (lane == 0) scales[t] = s.s;
+}
+
 // Rows of any width and start, one block each, read twice.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_any_kernel(const T* x, int64_t rows, int K, int8_t* codes, int pitch,
@@ -286,16 +308,33 @@ static int pitch_of(int K) { return (K + 15) & ~15; }
 static bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // Bytes copied to rows `pitch` apart, for codes whose rows do not start on 16 bytes.
+// A warp per row, four codes at a time: two neighbouring words of the source, shifted; the
+// row's first and last words byte by byte, so that no byte outside it is read.
 __global__ void __launch_bounds__(256) pitch_kernel(const int8_t* src, int64_t rows, int K, int8_t* dst, int pitch) {
+  const int lane = threadIdx.x & 31, words = (K + 3) / 4;
   dependency_wait();
-  const int64_t n = rows * K;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-    dst[i / K * pitch + i % K] = src[i];
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
+    const uint8_t* a = reinterpret_cast<const uint8_t*>(src) + r * K;
+    const int off = (int)(reinterpret_cast<uintptr_t>(a) & 3);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(a - off);
+    uint32_t* b = reinterpret_cast<uint32_t*>(dst + r * pitch);
+#pragma unroll 4
+    for (int c = lane; c < words; c += 32) {
+      uint32_t v = 0;
+      if (c > 0 && c < words - 2) {
+        v = __funnelshift_r(w[c], w[c + 1], 8 * off);
+      } else {
+        for (int j = 0; j < 4; ++j)
+          if (4 * c + j < K) v |= (uint32_t)a[4 * c + j] << (8 * j);
+      }
+      b[c] = v;
+    }
+  }
 }
 static cudaError_t pitched(const int8_t*& p, int64_t rows, int K, int8_t* copy, cudaStream_t s) {
   if (K % 16 == 0 && aligned(p, 16)) return cudaSuccess;
-  int64_t b = (rows * K + 2047) / 2048;
-  if (b > device_sm_count() * 16) b = device_sm_count() * 16;
+  int64_t b = (rows + 7) / 8;
+  if (b > device_sm_count() * 8) b = device_sm_count() * 8;
   const cudaError_t e = launch_after(pitch_kernel, dim3((unsigned)b), dim3(256), 0, s, p, rows, K, copy, pitch_of(K));
   p = copy;
   return e;
@@ -307,6 +346,10 @@ static cudaError_t quantize(const void* xv, int64_t rows, int K, int8_t* codes, 
   constexpr int N = Vec<T>::N;
   const int pitch = pitch_of(K);
   if (K % N != 0 || !aligned(x, 16) || K > 32 * N * 32) {
+    const dim3 warps((unsigned)((rows + 7) / 8));
+    if (K <= 256) return launch_after(quantize_odd_kernel<T, 8>, warps, dim3(256), 0, s, x, rows, K, codes, pitch, scales);
+    if (K <= 512) return launch_after(quantize_odd_kernel<T, 16>, warps, dim3(256), 0, s, x, rows, K, codes, pitch, scales);
+    if (K <= 1024) return launch_after(quantize_odd_kernel<T, 32>, warps, dim3(256), 0, s, x, rows, K, codes, pitch, scales);
     const int64_t most = (int64_t)device_sm_count() * 8;
     return launch_after(quantize_any_kernel<T>, dim3((unsigned)(rows < most ? rows : most)), dim3(256), 0, s, x, rows, K,
                         codes, pitch, scales);
