@@ -10,7 +10,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 HALF_ULP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
-SHAPES = [(128, 24), (7,), (1,), (255,), (256,), (257,), (3, 1001), (0,), (2, 5, 64), (4096,)]
+SHAPES = [(128, 25), (7,), (1,), (255,), (256,), (257,), (3, 1001), (0,), (2, 5, 64), (4096,)]
 H = dict(lr=3e-3, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.05)
 
 

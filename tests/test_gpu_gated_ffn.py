@@ -102,6 +102,27 @@ def test_against_64_bits(fms, dtype, rows, dim, hidden):
     assert torch.equal(fms.gated_ffn(x, wg, wu), got["h"])
 
 
+# Enough tiles for pairs of SMs, at widths that end inside a tile, inside a store's 64
+# columns and off 16 bytes; few rows and many columns, whose input gradient is summed in
+# parts; many rows and few columns, whose weights' gradients are.
+TILES = [(1500, 64, 1500), (900, 72, 2603), (1020, 136, 1067), (1301, 201, 1800), (100, 264, 2048), (2049, 72, 1161),
+         (9000, 40, 70), (700, 1000, 1601)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,dim,hidden", TILES)
+def test_tiles_against_64_bits(fms, dtype, rows, dim, hidden):
+    x, wg, wu, dh = make(rows, dim, hidden, dtype, rows + hidden)
+    check(run_all(fms, x, wg, wu, dh, "gelu"), reference(x, wg, wu, dh, "gelu"))
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])
+def test_activations_in_tiles(fms, act):
+    x, wg, wu, dh = make(1030, 64, 1600, torch.float16, 17)
+    x = (x.float() * 4).to(x.dtype)
+    check(run_all(fms, x, wg, wu, dh, act), reference(x, wg, wu, dh, act))
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])
 @pytest.mark.parametrize("rows", [1, 5, 140])
 def test_activations(fms, act, rows):

@@ -28,7 +28,7 @@ def codes32(x):
 
 
 def check(y, xc, xs, w, bias):
-    acc = xc @ w.codes.cpu().numpy().astype(np.int64).T
+    acc = xc.astype(np.float64) @ w.codes.cpu().numpy().astype(np.float64).T  # whole numbers below 2^53: exact
     v = acc * (xs.astype(np.float64)[:, None] * w.scales.cpu().numpy().astype(np.float64)[None, :])
     b = 0.0 if bias is None else bias.double().cpu().numpy()[None, :]
     bound = 3 * 2.0 ** -24 * (np.abs(v) + np.abs(b)) + HALF_ULP[y.dtype] * 1.01 * np.abs(v + b) + TINY[y.dtype]
@@ -48,6 +48,19 @@ def test_against_exact_sums(fms, dtype, rows, dim, out):
     x, w, b = make(fms, rows, dim, out, dtype, rows + dim + out)
     xc, xs = codes32(x)
     check(fms.int8_linear(x, w), xc, xs, w, None)
+    check(fms.int8_linear(x, w, bias=b), xc, xs, w, b)
+
+
+# Enough tiles for pairs of SMs, at widths that end inside a tile and off 16 bytes; rows of
+# codes and of features that do not start on 16 bytes.
+TILES = [(1500, 256, 3001), (1301, 101, 2600), (2600, 64, 1500), (1020, 1500, 2056), (999, 2051, 1100)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,dim,out", TILES)
+def test_tiles_against_exact_sums(fms, dtype, rows, dim, out):
+    x, w, b = make(fms, rows, dim, out, dtype, rows + out)
+    xc, xs = codes32(x)
     check(fms.int8_linear(x, w, bias=b), xc, xs, w, b)
 
 
