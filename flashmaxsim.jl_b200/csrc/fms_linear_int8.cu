@@ -9,7 +9,9 @@
 //
 // Up to FEW tokens one kernel quantises and multiplies on the CUDA cores (bound by
 // reading the weights once); more go through a quantising pass and the tcgen05
-// engine (kind::i8, scales in the epilogue).
+// engine (kind::i8, scales in the epilogue).  (One kernel that quantises into the MMA's
+// shared memory, for layers of up to 256 channels whose weights stay there, was between 18%
+// faster and 28% slower over 18944 to 180000 tokens, and no faster at 46080 x 768 -> 128.)
 #include "fms_gemm_tc.cuh"
 #include "fms_internal.h"
 
@@ -250,6 +252,7 @@ struct ScaleEpi {
     int64_t rows;
     int cols;
     int mapped;       // rows of y start on 16 bytes
+    int wide;         // sw and bias start on 16 bytes
   };
   template <int BN>
   struct Ahead {};
@@ -268,12 +271,35 @@ struct ScaleEpi {
       if (c + 1 == (half + 1) * (BN / 64)) release();
       const int col = t.n * BN + c * 32;
       float f[32];
-      // columns past the end take the last one's scale; they are not stored
+      // All lanes read the same scales and biases, so the loads are as wide as they may be:
+      // 32768 x 256 -> 1024 in bfloat16 44 us, by single values 50.
+      // Columns past the end take the last one's; they are not stored.
+      if (p.wide && col + 32 <= p.cols) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const int at = min(col + i, p.cols - 1);
-        f[i] = (sx * __ldg(p.sw + at)) * (float)(int32_t)v[i];
-        if (p.bias) f[i] += Tr<Y>::to(p.bias[at]);
+        for (int i = 0; i < 32; i += 4) {
+          const float4 w = __ldg(reinterpret_cast<const float4*>(p.sw + col + i));
+          f[i] = (sx * w.x) * (float)(int32_t)v[i];
+          f[i + 1] = (sx * w.y) * (float)(int32_t)v[i + 1];
+          f[i + 2] = (sx * w.z) * (float)(int32_t)v[i + 2];
+          f[i + 3] = (sx * w.w) * (float)(int32_t)v[i + 3];
+        }
+        if (p.bias) {
+          constexpr int N = Vec<Y>::N;
+#pragma unroll
+          for (int i = 0; i < 32; i += N) {
+            float b[N];
+            Vec<Y>::get(__ldg(reinterpret_cast<const uint4*>(p.bias + col + i)), b);
+#pragma unroll
+            for (int j = 0; j < N; ++j) f[i + j] += b[j];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int at = min(col + i, p.cols - 1);
+          f[i] = (sx * __ldg(p.sw + at)) * (float)(int32_t)v[i];
+          if (p.bias) f[i] += Tr<Y>::to(p.bias[at]);
+        }
       }
       // 128 bytes of a row at a time: every 32 columns in float32, every 64 in 16 bits
       constexpr int PER = 128 / sizeof(Y), GROUPS = BN >= 128 ? PER / 32 : 1;
@@ -429,6 +455,7 @@ static cudaError_t product(const int8_t* xc, const float* sx, const int8_t* wc, 
   e.y = (Y*)p.y;
   e.rows = p.rows;
   e.cols = p.C;
+  e.wide = aligned(p.sw, 16) && (!p.bias || aligned(p.bias, 16));
   e.mapped = p.C * sizeof(Y) % 16 == 0 && aligned(p.y, 16) &&
              gemm::make_map(&e.map, sizeof(Y) == 4 ? FMS_F32 : std::is_same<Y, __half>::value ? FMS_F16 : FMS_BF16, p.y, p.C,
                             p.rows, (int64_t)p.C * sizeof(Y), 32);

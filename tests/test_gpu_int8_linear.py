@@ -64,6 +64,50 @@ def test_tiles_against_exact_sums(fms, dtype, rows, dim, out):
     check(fms.int8_linear(x, w, bias=b), xc, xs, w, b)
 
 
+# Narrow layers over many tokens: whole and part tiles of tokens, widths inside a block of the
+# sum and at its end, outputs inside a tile and off 16 bytes; a token of zeros.
+NARROW = [(18944, 128, 128), (19000, 48, 64), (20001, 768, 128), (18951, 752, 100), (19072, 1024, 33), (40000, 512, 256),
+          (19100, 272, 200), (18945, 16, 1), (19333, 640, 65), (18944, 1040, 64), (18943, 256, 128), (57000, 144, 48)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,dim,out", NARROW)
+def test_narrow_against_exact_sums(fms, dtype, rows, dim, out):
+    x, w, b = make(fms, rows, dim, out, dtype, rows + dim + out)
+    x[rows - 3] = 0
+    xc, xs = codes32(x)
+    y = fms.int8_linear(x, w, bias=b)
+    check(y, xc, xs, w, b)
+    other = torch.float32 if dtype != torch.float32 else torch.bfloat16
+    check(fms.int8_linear(x, w, out_dtype=other), xc, xs, w, None)
+    assert torch.equal(y, fms.int8_linear(x, w, bias=b))
+    assert torch.equal(y[-70:], fms.int8_linear(x[-70:].contiguous(), w, bias=b))  # another tile's bits
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [60, 700])
+def test_scales_and_bias_off_16_bytes(fms, dtype, rows):
+    x, w, b = make(fms, rows, 192, 161, dtype, rows)
+    tail = fms.Int8Index(w.codes[1:].contiguous(), w.scales[1:])
+    xc, xs = codes32(x)
+    y = fms.int8_linear(x, tail, bias=b[1:])
+    check(y, xc, xs, tail, b[1:])
+    whole = fms.Int8Index(tail.codes, tail.scales.clone())
+    for bias in (b[1:], b[1:].clone()):
+        assert torch.equal(fms.int8_linear(x, whole, bias=bias), y)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_narrow_layer_keeps_a_bad_token_to_itself(fms, bad):
+    x, w, b = make(fms, 19000, 256, 96, torch.bfloat16)
+    good = fms.int8_linear(x, w, bias=b)
+    x[18000, 77] = bad
+    y = fms.int8_linear(x, w, bias=b)
+    assert y[18000].isnan().all()
+    keep = torch.arange(19000, device="cuda") != 18000
+    assert torch.equal(y[keep], good[keep])
+
+
 @pytest.mark.parametrize("rows", [1, 6, 40, 200])
 def test_quantised_features(fms, rows):
     """An Int8Index of features, scores in every type; equal to the float call on its codes."""
