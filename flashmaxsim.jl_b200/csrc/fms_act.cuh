@@ -41,8 +41,8 @@ __device__ __forceinline__ void act_eval2(float2 g, float2& a, float2& da) {
   if (ACT == FMS_ACT_SILU) {
     const float2 s = logistic2(__fmul2_rn(g, pair(-LOG2E)));
     a = __fmul2_rn(g, s);
-    // s (1 + g (1 - s)) = s + a - a s
-    if (DERIV) da = __ffma2_rn(make_float2(-a.x, -a.y), s, __fadd2_rn(s, a));
+    // s (1 + g (1 - s)) = s + a (1 - s); with 1 - s taken first, s + a does not round to a
+    if (DERIV) da = __ffma2_rn(a, __fadd2_rn(pair(1.f), make_float2(-s.x, -s.y)), s);
   } else if (ACT == FMS_ACT_GELU) {
     // Phi(-|g|) = q = t (a1 + t (a2 + ...)) e^(-g^2/2) / 2, t = 1 / (1 + p |g| / sqrt 2)
     // (Abramowitz and Stegun 7.1.26, off by 0.75e-7 at most); past 30 it is zero.
