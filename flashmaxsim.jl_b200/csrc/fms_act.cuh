@@ -72,9 +72,10 @@ __device__ __forceinline__ void act_eval2(float2 g, float2& a, float2& da) {
     const float2 s = logistic2(y);
     a = __fmul2_rn(g, s);
     if (DERIV) {
-      // s + g s (1 - s) 2 y',  y' = k (1 + 3 c g^2)
-      const float2 d = __ffma2_rn(g2, pair(6.f * K * C), pair(2.f * K));
-      da = __ffma2_rn(__fmul2_rn(a, d), __fadd2_rn(pair(1.f), make_float2(-s.x, -s.y)), s);
+      // s + g s (1 - s) 2 y',  y' = k (1 + 3 c g^2).  From |g| = 10 on s (1 - s) is
+      // below 2^-125 or zero: g^2 may end at 100, so that no infinity meets that zero.
+      const float2 d = __ffma2_rn(make_float2(fminf(g2.x, 100.f), fminf(g2.y, 100.f)), pair(6.f * K * C), pair(2.f * K));
+      da = __ffma2_rn(__fmul2_rn(a, __fadd2_rn(pair(1.f), make_float2(-s.x, -s.y))), d, s);
     }
   } else {  // FMS_ACT_RELU; a NaN stays one
     a = make_float2(max_nan(g.x, 0.f), max_nan(g.y, 0.f));

@@ -15,7 +15,7 @@ def grads(fms, x, wg, wu, act):
     return (h.detach(), *torch.autograd.grad(h, leaves, torch.ones_like(h)))
 
 
-@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])
 def test_derivative_is_one_or_zero(fms, act):
     """x = 1 and w_up = 1: dw_gate is the derivative itself, dw_up the activation; at -40 both
     are below 40 e^-40 < 1e-15."""
@@ -29,7 +29,7 @@ def test_derivative_is_one_or_zero(fms, act):
     assert dx.item() == pytest.approx(2 * float((wg * on).double().sum()), rel=2.0 ** -7)
 
 
-@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
 def test_derivative_of_thousands_in_float16(fms, act):
     """g between 1e3 and 8e4 with a fraction: dw_gate = x dg with dg = u rounded to float16,
     two roundings of half a unit (2^-11) and 2^-18 for the derivative."""
