@@ -39,3 +39,28 @@ def test_derivative_of_thousands_in_float16(fms, act):
     _, _, dg, _ = grads(fms, x, wg, wu, act)
     want = float(x.double()) ** 2 * wu.double()
     assert ((dg.double() - want).abs() <= (2 * 2.0 ** -11 + 2.0 ** -18) * 1.001 * want).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_the_small_side_of_gelu(fms, dtype, rows):
+    """g from -12.5 to 0 and to 4, where Phi(g) falls to 4e-36: h and the derivative are right
+    relative to their own size.  2^-13 of Phi(g) covers the fit's 6.1e-5 with the float32
+    roundings around it, against half a unit of the last place (float16: of its smallest)."""
+    wg = torch.cat([torch.linspace(-12.5, 0, 400, device="cuda"), torch.linspace(0, 4, 100, device="cuda")]).to(dtype)[:, None]
+    one = torch.ones_like(wg)
+    x = torch.zeros(rows, 1, device="cuda", dtype=dtype)
+    x[-1] = 1
+    leaf = wg.clone().requires_grad_()
+    h = fms.gated_ffn(x, leaf, one, act="gelu")
+    dh = torch.zeros_like(h)
+    dh[-1] = 1
+    dg, = torch.autograd.grad(h, leaf, dh)
+    g = wg.double()[:, 0]
+    ndtr = lambda v: 0.5 * torch.erfc(-v * 0.5 ** 0.5)  # noqa: E731  (torch's own is 1 + erf: nothing below 1e-16)
+    cdf, slope = ndtr(g), g * torch.exp(-g * g / 2) / (2 * torch.pi) ** 0.5
+    hu, tiny = (2.0 ** -11, 2.0 ** -25) if dtype == torch.float16 else (2.0 ** -8, 2.0 ** -134)
+    near = torch.minimum(cdf, ndtr(-g))
+    for got, want, size in ((h[-1], g * cdf, g.abs() * near), (dg[:, 0], cdf + slope, near + slope.abs())):
+        off = (got.double() - want).abs() - (2.0 ** -13 * size + 2.0 ** -20 * want.abs() + hu * 1.01 * want.abs() + tiny)
+        assert not (off > 0).any(), (g[off > 0], got[off > 0], want[off > 0])
