@@ -121,19 +121,22 @@ __device__ __forceinline__ void store(T* row, int tid, int tpr, int D, const flo
   }
 }
 
-// The same of a weight, bias or gate (in T or float32) from element `at` on.
-template <typename T, int VEC, int N>
+// The same of a weight, bias or gate (in T or float32) from element `at` on.  WIDE: it
+// starts on 16 bytes where it is in T.  (Only its own loads depend on that: how a row is
+// read, and so what it adds up to, must not.)
+template <bool WIDE, typename T, int VEC, int N>
 __device__ __forceinline__ void load_vec(const void* p, int vdt, int64_t at, int tid, int tpr, int D, float2 (&f)[N]) {
-  if (sizeof(T) == 4 || vdt != FMS_F32) {
+  if (WIDE && (sizeof(T) == 4 || vdt != FMS_F32)) {
     Raw<T, VEC, N> r;
     r.load(static_cast<const T*>(p) + at, tid, tpr, D);
     r.get(f);
   } else {
     const float* q = static_cast<const float*>(p) + at;
+    const T* u = static_cast<const T*>(p) + at;
 #pragma unroll
     for (int e = 0; e < 2 * N; ++e) {
       const int c = (e / VEC * tpr + tid) * VEC + e % VEC;
-      const float v = c < D ? __ldg(q + c) : 0.f;
+      const float v = c >= D ? 0.f : WIDE || vdt == FMS_F32 ? __ldg(q + c) : Tr<T>::to(u[c]);
       if (e & 1) f[e >> 1].y = v;
       else f[e >> 1].x = v;
     }
@@ -183,7 +186,7 @@ struct RowSum {
 };
 
 // One row per warp (WARP, rows of up to 1024) or block; a thread holds N pairs.
-template <typename T, int VEC, int N, bool WARP>
+template <typename T, int VEC, int N, bool WIDE, bool WARP>
 __global__ void __launch_bounds__(WARP ? 128 : 1024) forward_kernel(Params p) {
   __shared__ float part[2][MAX_WARPS];
   RowSum<WARP, 1> sum{part};
@@ -234,12 +237,12 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) forward_kernel(Params p) {
   };
   // v = (a - mean) rstd w + b
   auto apply = [&](float2 (&a)[N], float mean, float rstd, const void* wv, const void* bv) {
-    load_vec<T, VEC, N>(wv, p.vdt, 0, tid, tpr, D, w);
+    load_vec<WIDE, T, VEC, N>(wv, p.vdt, 0, tid, tpr, D, w);
     const float shift = -mean * rstd;
 #pragma unroll
     for (int k = 0; k < N; ++k) a[k] = __fmul2_rn(__ffma2_rn(a[k], two(rstd), two(shift)), w[k]);
     if (bv) {
-      load_vec<T, VEC, N>(bv, p.vdt, 0, tid, tpr, D, w);
+      load_vec<WIDE, T, VEC, N>(bv, p.vdt, 0, tid, tpr, D, w);
 #pragma unroll
       for (int k = 0; k < N; ++k) a[k] = __fadd2_rn(a[k], w[k]);
     }
@@ -248,7 +251,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) forward_kernel(Params p) {
   stats(v, mh, rh);
   apply(v, mh, rh, p.w_post, p.b_post);
   if (p.gate) {
-    load_vec<T, VEC, N>(p.gate, p.vdt, (r / p.per) * D, tid, tpr, D, w);
+    load_vec<WIDE, T, VEC, N>(p.gate, p.vdt, (r / p.per) * D, tid, tpr, D, w);
 #pragma unroll
     for (int k = 0; k < N; ++k) v[k] = __fmul2_rn(v[k], w[k]);
   }
@@ -281,7 +284,7 @@ __device__ __forceinline__ void put_sums(float* o, int tid, int tpr, int D, cons
 // A run of rows per block, a row at a time with the next one's loads in flight; a thread
 // owns the same N pairs of columns in every row and keeps their sums in registers.
 // BIAS: S0 and T0 are wanted too.
-template <typename T, int VEC, int N, bool BIAS>
+template <typename T, int VEC, int N, bool WIDE, bool BIAS>
 __global__ void __launch_bounds__(512) backward_kernel(Params p) {
   __shared__ float part[2][MAX_WARPS * 2];
   RowSum<false, 2> sum{part};
@@ -293,16 +296,16 @@ __global__ void __launch_bounds__(512) backward_kernel(Params p) {
   float* const outT = p.part + 2 * (p.blocks + p.groups) * D;
   float2 gw[N], gb[N], wp[N];  // gate w_post, gate b_post, w_pre
   float2 S1[N], T1[N], S0[N], T0[N];
-  load_vec<T, VEC, N>(p.w_pre, p.vdt, 0, tid, tpr, D, wp);
+  load_vec<WIDE, T, VEC, N>(p.w_pre, p.vdt, 0, tid, tpr, D, wp);
 #pragma unroll
   for (int k = 0; k < N; ++k) S1[k] = T1[k] = S0[k] = T0[k] = gb[k] = two(0.f);
   int64_t group = r0 / p.per;
   auto enter = [&]() {
-    load_vec<T, VEC, N>(p.w_post, p.vdt, 0, tid, tpr, D, gw);
-    if (BIAS && p.b_post) load_vec<T, VEC, N>(p.b_post, p.vdt, 0, tid, tpr, D, gb);
+    load_vec<WIDE, T, VEC, N>(p.w_post, p.vdt, 0, tid, tpr, D, gw);
+    if (BIAS && p.b_post) load_vec<WIDE, T, VEC, N>(p.b_post, p.vdt, 0, tid, tpr, D, gb);
     if (p.gate) {
       float2 g[N];
-      load_vec<T, VEC, N>(p.gate, p.vdt, group * D, tid, tpr, D, g);
+      load_vec<WIDE, T, VEC, N>(p.gate, p.vdt, group * D, tid, tpr, D, g);
 #pragma unroll
       for (int k = 0; k < N; ++k) gw[k] = __fmul2_rn(gw[k], g[k]), gb[k] = __fmul2_rn(gb[k], g[k]);
     }
@@ -478,57 +481,60 @@ static int parts_of(int64_t groups, int64_t blocks) {
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <typename T, int VEC, int N, bool WARP>
+template <typename T, int VEC, int N, bool WIDE, bool WARP>
 static void forward(const Params& p, cudaStream_t s) {
   if constexpr (WARP) {
-    launch_after(forward_kernel<T, VEC, N, true>, dim3((unsigned)((p.rows + 3) / 4)), dim3(128), 0, s, p);
+    launch_after(forward_kernel<T, VEC, N, WIDE, true>, dim3((unsigned)((p.rows + 3) / 4)), dim3(128), 0, s, p);
   } else {
     const int tpr = (p.dim + 2 * N * 32 - 1) / (2 * N * 32) * 32;
-    launch_after(forward_kernel<T, VEC, N, false>, dim3((unsigned)p.rows), dim3(tpr), 0, s, p);
+    launch_after(forward_kernel<T, VEC, N, WIDE, false>, dim3((unsigned)p.rows), dim3(tpr), 0, s, p);
   }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool WIDE>
 static void run_forward(const Params& p, cudaStream_t s) {
-  if (p.dim <= 256) forward<T, VEC, 4, true>(p, s);
-  else if (p.dim <= 512) forward<T, VEC, 8, true>(p, s);
-  else if (p.dim <= 768) forward<T, VEC, 12, true>(p, s);
-  else if (p.dim <= 1024) forward<T, VEC, 16, true>(p, s);
-  else if (p.dim <= 8192) forward<T, VEC, 4, false>(p, s);
-  else forward<T, VEC, 8, false>(p, s);
+  if (p.dim <= 256) forward<T, VEC, 4, WIDE, true>(p, s);
+  else if (p.dim <= 512) forward<T, VEC, 8, WIDE, true>(p, s);
+  else if (p.dim <= 768) forward<T, VEC, 12, WIDE, true>(p, s);
+  else if (p.dim <= 1024) forward<T, VEC, 16, WIDE, true>(p, s);
+  else if (p.dim <= 8192) forward<T, VEC, 4, WIDE, false>(p, s);
+  else forward<T, VEC, 8, WIDE, false>(p, s);
 }
 
-template <typename T, int VEC, int N, bool BIAS>
+template <typename T, int VEC, int N, bool WIDE, bool BIAS>
 static void backward(const Params& p, cudaStream_t s) {
   const int tpr = (p.dim + 2 * N * 32 - 1) / (2 * N * 32) * 32;
-  launch_after(backward_kernel<T, VEC, N, BIAS>, dim3((unsigned)p.blocks), dim3(tpr), 0, s, p);
+  launch_after(backward_kernel<T, VEC, N, WIDE, BIAS>, dim3((unsigned)p.blocks), dim3(tpr), 0, s, p);
 }
 
-template <typename T, int VEC, bool BIAS>
+template <typename T, int VEC, bool WIDE, bool BIAS>
 static void run_backward(const Params& p, cudaStream_t s) {
-  if (p.dim <= 4096) backward<T, VEC, 4, BIAS>(p, s);
-  else if (p.dim <= 8192) backward<T, VEC, 8, BIAS>(p, s);
-  else backward<T, VEC, 16, BIAS>(p, s);
+  if (p.dim <= 4096) backward<T, VEC, 4, WIDE, BIAS>(p, s);
+  else if (p.dim <= 8192) backward<T, VEC, 8, WIDE, BIAS>(p, s);
+  else backward<T, VEC, 16, WIDE, BIAS>(p, s);
 }
 
 template <typename T>
 static void run(const Params& p, bool bwd, cudaStream_t s) {
   constexpr int VEC = 16 / sizeof(T);
-  const bool vec = p.dim % VEC == 0 && aligned16(p.x) && aligned16(p.h) && aligned16(p.w_post) && aligned16(p.b_post) &&
-                   aligned16(p.w_pre) && aligned16(p.b_pre) && aligned16(p.gate) &&
+  const bool wide = aligned16(p.w_post) && aligned16(p.b_post) && aligned16(p.w_pre) && aligned16(p.b_pre) && aligned16(p.gate);
+  const bool vec = p.dim % VEC == 0 && aligned16(p.x) && aligned16(p.h) &&
                    (bwd ? aligned16(p.dz) && aligned16(p.dy) && aligned16(p.dx) && aligned16(p.dh)
                         : aligned16(p.z) && aligned16(p.y));
   if (!bwd) {
-    if (vec) run_forward<T, VEC>(p, s);
-    else run_forward<T, 1>(p, s);
+    if (vec && wide) run_forward<T, VEC, true>(p, s);
+    else if (vec) run_forward<T, VEC, false>(p, s);
+    else run_forward<T, 1, true>(p, s);
     return;
   }
   const bool bias = p.b_post || p.db_post || p.db_pre;
   if (p.rows > 0) {
-    if (vec && bias) run_backward<T, VEC, true>(p, s);
-    else if (vec) run_backward<T, VEC, false>(p, s);
-    else if (bias) run_backward<T, 1, true>(p, s);
-    else run_backward<T, 1, false>(p, s);
+    if (vec && wide && bias) run_backward<T, VEC, true, true>(p, s);
+    else if (vec && wide) run_backward<T, VEC, true, false>(p, s);
+    else if (vec && bias) run_backward<T, VEC, false, true>(p, s);
+    else if (vec) run_backward<T, VEC, false, false>(p, s);
+    else if (bias) run_backward<T, 1, true, true>(p, s);
+    else run_backward<T, 1, true, false>(p, s);
   }
   const int parts = parts_of(p.groups, p.blocks);
   float* sums = p.part + (4 * p.blocks + 2 * p.groups) * p.dim;
