@@ -204,8 +204,11 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) forward_kernel(Params p) {
     h.get(v);
     x.get(z);
   }
-  // mean, and the reciprocal deviation of the centred values (two passes over registers)
-  auto stats = [&](float2 (&a)[N], float& mean, float& rstd) {
+  // Takes the mean off the values and gives it and their reciprocal deviation (two passes
+  // over registers).  The mean comes off before that factor goes on, and is the quotient
+  // that rounds right, so that a row of one value is zero whatever 1 / sqrt(eps) multiplies
+  // it by; the values past the row's end are no zeros afterwards.
+  auto centre = [&](float2 (&a)[N], float& mean, float& rstd) {
     float s[1];
     mean = 0.f;
     if (p.layer) {
@@ -215,32 +218,31 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) forward_kernel(Params p) {
       s[0] = t.x + t.y;
       sum(s);
       mean = s[0] * inv_d;
+      mean = fmaf(fmaf(-mean, (float)D, s[0]), inv_d, mean);  // the quotient, by its remainder
+#pragma unroll
+      for (int k = 0; k < N; ++k) a[k] = __fadd2_rn(a[k], two(-mean));
     }
     float2 t = two(0.f);
 #pragma unroll
     for (int i = 0; i < 2 * N / VEC; ++i)
-      if ((i * tpr + tid) * VEC < D) {  // the values past the row's end are no zeros once centred
+      if ((i * tpr + tid) * VEC < D) {
         if constexpr (VEC == 1) {
-          const float d = (i & 1 ? a[i >> 1].y : a[i >> 1].x) - mean;
+          const float d = i & 1 ? a[i >> 1].y : a[i >> 1].x;
           t.x = fmaf(d, d, t.x);
         } else {
 #pragma unroll
-          for (int k = 0; k < VEC / 2; ++k) {
-            const float2 d = __fadd2_rn(a[i * (VEC / 2) + k], two(-mean));
-            t = __ffma2_rn(d, d, t);
-          }
+          for (int k = 0; k < VEC / 2; ++k) t = __ffma2_rn(a[i * (VEC / 2) + k], a[i * (VEC / 2) + k], t);
         }
       }
     s[0] = t.x + t.y;
     sum(s);
     rstd = rsqrtf(s[0] * inv_d + p.eps);
   };
-  // v = (a - mean) rstd w + b
-  auto apply = [&](float2 (&a)[N], float mean, float rstd, const void* wv, const void* bv) {
+  // a = a rstd w + b
+  auto apply = [&](float2 (&a)[N], float rstd, const void* wv, const void* bv) {
     load_vec<WIDE, T, VEC, N>(wv, p.vdt, 0, tid, tpr, D, w);
-    const float shift = -mean * rstd;
 #pragma unroll
-    for (int k = 0; k < N; ++k) a[k] = __fmul2_rn(__ffma2_rn(a[k], two(rstd), two(shift)), w[k]);
+    for (int k = 0; k < N; ++k) a[k] = __fmul2_rn(__fmul2_rn(a[k], two(rstd)), w[k]);
     if (bv) {
       load_vec<WIDE, T, VEC, N>(bv, p.vdt, 0, tid, tpr, D, w);
 #pragma unroll
@@ -248,8 +250,8 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) forward_kernel(Params p) {
     }
   };
   float mh, rh, mz, rz;
-  stats(v, mh, rh);
-  apply(v, mh, rh, p.w_post, p.b_post);
+  centre(v, mh, rh);
+  apply(v, rh, p.w_post, p.b_post);
   if (p.gate) {
     load_vec<WIDE, T, VEC, N>(p.gate, p.vdt, (r / p.per) * D, tid, tpr, D, w);
 #pragma unroll
@@ -258,8 +260,8 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) forward_kernel(Params p) {
 #pragma unroll
   for (int k = 0; k < N; ++k) z[k] = __ffma2_rn(z[k], two(p.scale), v[k]);
   store<T, VEC, N>(static_cast<T*>(p.z) + r * D, tid, tpr, D, z);
-  stats(z, mz, rz);
-  apply(z, mz, rz, p.w_pre, p.b_pre);
+  centre(z, mz, rz);
+  apply(z, rz, p.w_pre, p.b_pre);
   store<T, VEC, N>(static_cast<T*>(p.y) + r * D, tid, tpr, D, z);
   if (p.stats && tid == 0) {
     p.stats[r] = mh;
@@ -283,9 +285,11 @@ __device__ __forceinline__ void put_sums(float* o, int tid, int tpr, int D, cons
 
 // A run of rows per block, a row at a time with the next one's loads in flight; a thread
 // owns the same N pairs of columns in every row and keeps their sums in registers.
-// BIAS: S0 and T0 are wanted too.
+// BIAS: S0 and T0 are wanted too.  One block an SM is asked for by name: left to itself
+// the compiler gave the widest rows 32 or 64 registers a thread and spilled the rest
+// (11520 x 5120 bf16 layer 1320 us, 513 with 128 registers).
 template <typename T, int VEC, int N, bool WIDE, bool BIAS>
-__global__ void __launch_bounds__(512) backward_kernel(Params p) {
+__global__ void __launch_bounds__(512, 1) backward_kernel(Params p) {
   __shared__ float part[2][MAX_WARPS * 2];
   RowSum<false, 2> sum{part};
   dependency_wait();
@@ -346,14 +350,14 @@ __global__ void __launch_bounds__(512) backward_kernel(Params p) {
     if (p.dy) ry.get(dy);
     if (p.dz) rd.get(d);
     if (r + 1 < r1) fetch(r + 1);
-    const float2 nh = two(-mh * rh), nz = two(-mz * rz);
+    const float2 nh = two(-mh), nz = two(-mz);
     float2 s0 = two(0.f), s1 = two(0.f);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      hh[k] = __ffma2_rn(hh[k], two(rh), nh);
+      hh[k] = __fmul2_rn(__fadd2_rn(hh[k], nh), two(rh));
       float2 z = __ffma2_rn(hh[k], gw[k], __fmul2_rn(zh[k], two(p.scale)));
       if (BIAS) z = __fadd2_rn(z, gb[k]);
-      zh[k] = __ffma2_rn(z, two(rz), nz);
+      zh[k] = __fmul2_rn(__fadd2_rn(z, nz), two(rz));
       const float2 t = __fmul2_rn(dy[k], wp[k]);  // 0 past the row's end
       s0 = __ffma2_rn(t, zh[k], s0);
       s1 = __fadd2_rn(s1, t);
