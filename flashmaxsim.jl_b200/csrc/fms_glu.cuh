@@ -228,8 +228,9 @@ struct Pitches {
   }
 };
 // Pairs of elements at a time: a row that starts on an odd element takes each pair from two
-// neighbouring words (copies are written in whole pairs: ld is even, what lies past n in a
-// row is never read as an element).
+// neighbouring words, its first and last pair by themselves, so that nothing outside the row
+// is read (copies are written in whole pairs: ld is even, what lies past n in a row is never
+// read as an element).
 static __global__ void __launch_bounds__(256) pitch_kernel(const Pitches p) {
   dependency_wait();
   const Pitch& j = p.m[blockIdx.y];
@@ -244,7 +245,8 @@ static __global__ void __launch_bounds__(256) pitch_kernel(const Pitches p) {
     } else {
       const uint32_t* w = reinterpret_cast<const uint32_t*>(a - 1);
 #pragma unroll 8
-      for (int c = lane; c < words; c += 32) b[c] = __funnelshift_r(w[c], w[c + 1], 16);
+      for (int c = lane; c < words; c += 32)
+        b[c] = c > 0 && c < words - 1 ? __funnelshift_r(w[c], w[c + 1], 16) : a[2 * c] | (uint32_t)a[2 * c + 1] << 16;
     }
     if (lane == 0 && j.n % 2 != 0) b[words] = a[j.n - 1];  // the last element, alone
   }
