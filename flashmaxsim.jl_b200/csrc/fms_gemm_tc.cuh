@@ -176,10 +176,11 @@ __device__ __forceinline__ uint64_t desc(uint32_t saddr) {
   return d;
 }
 
-// Health flag of this file's kernels (one per translation unit): a wait gave up.
+// Health flag of this file's kernels: a wait gave up.  The flag and its reader are each
+// translation unit's own.
 static __device__ int g_error = 0;
 
-inline int read_error(int reset) {
+static inline int read_error(int reset) {
   int v = 0;
   cudaError_t e = cudaMemcpyFromSymbol(&v, g_error, sizeof(int));
   if (e == cudaSuccess && reset) {
