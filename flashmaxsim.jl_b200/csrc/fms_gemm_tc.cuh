@@ -16,7 +16,7 @@
 // warps 2-9 drain accumulators: the subpartition a warp may read is its id mod 4,
 // so each subpartition has two warps, one for each half of the columns.  Every
 // wait is bounded: it gives up after two seconds, raises the health flag and lets
-// all roles leave.
+// all roles leave, once the copies and products in flight have ended (bounded as well).
 #pragma once
 #include <cuda.h>
 
@@ -90,6 +90,13 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
         return false;
       }
     }
+  }
+}
+
+// After a wait gave up: until the phase completes, the abort flag notwithstanding, or 10 ms.
+__device__ __forceinline__ void settle(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = ptx::globaltimer_ns();
+  while (!try_wait_cluster(bar, parity) && ptx::globaltimer_ns() - t0 < 10000000ull) {
   }
 }
 
@@ -319,10 +326,17 @@ kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensor
     // The ring is left to nobody's writes: wait (bounded) for the copies in flight.
     // In the leader every stage's barrier completes when both CTAs' copies have landed;
     // the other CTA's stages are released by the leader's commits.
+    const int next = s;
+    const uint32_t lap = ph;
     for (int i = 0; ok && i < R::STAGES; ++i) {
       ok = __all_sync(0xffffffffu, wait(&empty[s], ph ^ 1, &abort_s));
       if (++s == R::STAGES) s = 0, ph ^= 1;
     }
+    // Where a wait gave up there may be no more commits: the leader waits for each stage's
+    // last copies.  The other CTA, which cannot ask for them, stays until the leader is at
+    // the cluster's last barrier.
+    if (!ok && rk == 0)
+      for (int i = 0; i < R::STAGES; ++i) settle(&full[i], i < next ? lap : lap ^ 1);
   } else if (warp == 1 && rank == 0) {
     // ------------------------------------------------------------ MMA
     // The whole warp runs the loop, so that descriptors stay in uniform registers; one
@@ -355,6 +369,12 @@ kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensor
       if (elect_one()) commit<CG>(&accf[buf]);
       __syncwarp();
       if (++buf == 2) buf = 0, bph ^= 1;
+    }
+    // A wait gave up: the products in flight still read shared memory and write TMEM.
+    if (__any_sync(0xffffffffu, abort_s != 0)) {
+      if (elect_one()) commit<CG>(&accf[buf]);
+      __syncwarp();
+      settle(&accf[buf], bph);
     }
   } else if (warp >= 2) {
     // ------------------------------------------------------------ epilogue
