@@ -486,72 +486,69 @@ static int parts_of(int64_t groups, int64_t blocks) {
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <typename T, int VEC, int N, bool WIDE, bool WARP>
-static void forward(const Params& p, cudaStream_t s) {
+static cudaError_t forward(const Params& p, cudaStream_t s) {
   if constexpr (WARP) {
-    launch_after(forward_kernel<T, VEC, N, WIDE, true>, dim3((unsigned)((p.rows + 3) / 4)), dim3(128), 0, s, p);
+    return launch_after(forward_kernel<T, VEC, N, WIDE, true>, dim3((unsigned)((p.rows + 3) / 4)), dim3(128), 0, s, p);
   } else {
     const int tpr = (p.dim + 2 * N * 32 - 1) / (2 * N * 32) * 32;
-    launch_after(forward_kernel<T, VEC, N, WIDE, false>, dim3((unsigned)p.rows), dim3(tpr), 0, s, p);
+    return launch_after(forward_kernel<T, VEC, N, WIDE, false>, dim3((unsigned)p.rows), dim3(tpr), 0, s, p);
   }
 }
 
 template <typename T, int VEC, bool WIDE>
-static void run_forward(const Params& p, cudaStream_t s) {
-  if (p.dim <= 256) forward<T, VEC, 4, WIDE, true>(p, s);
-  else if (p.dim <= 512) forward<T, VEC, 8, WIDE, true>(p, s);
-  else if (p.dim <= 768) forward<T, VEC, 12, WIDE, true>(p, s);
-  else if (p.dim <= 1024) forward<T, VEC, 16, WIDE, true>(p, s);
-  else if (p.dim <= 8192) forward<T, VEC, 4, WIDE, false>(p, s);
-  else forward<T, VEC, 8, WIDE, false>(p, s);
+static cudaError_t run_forward(const Params& p, cudaStream_t s) {
+  if (p.dim <= 256) return forward<T, VEC, 4, WIDE, true>(p, s);
+  if (p.dim <= 512) return forward<T, VEC, 8, WIDE, true>(p, s);
+  if (p.dim <= 768) return forward<T, VEC, 12, WIDE, true>(p, s);
+  if (p.dim <= 1024) return forward<T, VEC, 16, WIDE, true>(p, s);
+  if (p.dim <= 8192) return forward<T, VEC, 4, WIDE, false>(p, s);
+  return forward<T, VEC, 8, WIDE, false>(p, s);
 }
 
 template <typename T, int VEC, int N, bool WIDE, bool BIAS>
-static void backward(const Params& p, cudaStream_t s) {
+static cudaError_t backward(const Params& p, cudaStream_t s) {
   const int tpr = (p.dim + 2 * N * 32 - 1) / (2 * N * 32) * 32;
-  launch_after(backward_kernel<T, VEC, N, WIDE, BIAS>, dim3((unsigned)p.blocks), dim3(tpr), 0, s, p);
+  return launch_after(backward_kernel<T, VEC, N, WIDE, BIAS>, dim3((unsigned)p.blocks), dim3(tpr), 0, s, p);
 }
 
 template <typename T, int VEC, bool WIDE, bool BIAS>
-static void run_backward(const Params& p, cudaStream_t s) {
-  if (p.dim <= 4096) backward<T, VEC, 4, WIDE, BIAS>(p, s);
-  else if (p.dim <= 8192) backward<T, VEC, 8, WIDE, BIAS>(p, s);
-  else backward<T, VEC, 16, WIDE, BIAS>(p, s);
+static cudaError_t run_backward(const Params& p, cudaStream_t s) {
+  if (p.dim <= 4096) return backward<T, VEC, 4, WIDE, BIAS>(p, s);
+  if (p.dim <= 8192) return backward<T, VEC, 8, WIDE, BIAS>(p, s);
+  return backward<T, VEC, 16, WIDE, BIAS>(p, s);
 }
 
 template <typename T>
-static void run(const Params& p, bool bwd, cudaStream_t s) {
+static cudaError_t run(const Params& p, bool bwd, cudaStream_t s) {
   constexpr int VEC = 16 / sizeof(T);
   const bool wide = aligned16(p.w_post) && aligned16(p.b_post) && aligned16(p.w_pre) && aligned16(p.b_pre) && aligned16(p.gate);
   const bool vec = p.dim % VEC == 0 && aligned16(p.x) && aligned16(p.h) &&
                    (bwd ? aligned16(p.dz) && aligned16(p.dy) && aligned16(p.dx) && aligned16(p.dh)
                         : aligned16(p.z) && aligned16(p.y));
-  if (!bwd) {
-    if (vec && wide) run_forward<T, VEC, true>(p, s);
-    else if (vec) run_forward<T, VEC, false>(p, s);
-    else run_forward<T, 1, true>(p, s);
-    return;
-  }
+  if (!bwd)
+    return vec && wide ? run_forward<T, VEC, true>(p, s)
+           : vec       ? run_forward<T, VEC, false>(p, s)
+                       : run_forward<T, 1, true>(p, s);
   const bool bias = p.b_post || p.db_post || p.db_pre;
+  cudaError_t e = cudaSuccess;
   if (p.rows > 0) {
-    if (vec && wide && bias) run_backward<T, VEC, true, true>(p, s);
-    else if (vec && wide) run_backward<T, VEC, true, false>(p, s);
-    else if (vec && bias) run_backward<T, VEC, false, true>(p, s);
-    else if (vec) run_backward<T, VEC, false, false>(p, s);
-    else if (bias) run_backward<T, 1, true, true>(p, s);
-    else run_backward<T, 1, true, false>(p, s);
+    if (vec && wide) e = bias ? run_backward<T, VEC, true, true>(p, s) : run_backward<T, VEC, true, false>(p, s);
+    else if (vec) e = bias ? run_backward<T, VEC, false, true>(p, s) : run_backward<T, VEC, false, false>(p, s);
+    else e = bias ? run_backward<T, 1, true, true>(p, s) : run_backward<T, 1, true, false>(p, s);
   }
+  if (e != cudaSuccess) return e;
   const int parts = parts_of(p.groups, p.blocks);
   float* sums = p.part + (4 * p.blocks + 2 * p.groups) * p.dim;
   const dim3 grid((unsigned)((p.dim + 31) / 32), (unsigned)parts);
-  launch_after(bias ? gather_kernel<true> : gather_kernel<false>, grid, dim3(1024), 0, s, p, sums);
-  launch_after(finish_kernel, dim3((unsigned)((p.dim + 127) / 128)), dim3(128), 0, s, p, (const float*)sums, parts);
+  e = launch_after(bias ? gather_kernel<true> : gather_kernel<false>, grid, dim3(1024), 0, s, p, sums);
+  if (e != cudaSuccess) return e;
+  return launch_after(finish_kernel, dim3((unsigned)((p.dim + 127) / 128)), dim3(128), 0, s, p, (const float*)sums, parts);
 }
 
 static int launch(int dtype, const Params& p, bool bwd, cudaStream_t s) {
-  if (dtype == FMS_F32) run<float>(p, bwd, s);
-  else if (dtype == FMS_F16) run<__half>(p, bwd, s);
-  else run<__nv_bfloat16>(p, bwd, s);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = dtype == FMS_F32   ? run<float>(p, bwd, s)
+                        : dtype == FMS_F16 ? run<__half>(p, bwd, s)
+                                           : run<__nv_bfloat16>(p, bwd, s);
   return e == cudaSuccess ? FMS_OK : (int)e;
 }
 
