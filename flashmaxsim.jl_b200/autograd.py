@@ -8,8 +8,10 @@ INT8 MaxSim is forward-only (rrule.jl:140-167).
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import layouts as L
+from .errors import ArgumentError
 from .packed import PackedSeq
 
 
@@ -138,6 +140,11 @@ class _Varlen(torch.autograd.Function):
 
 
 def needs_grad(*ts) -> bool:
+    """Whether a backward pass is wanted.  Tensors with a forward-mode tangent are refused:
+    the kernels have none, and it would be lost."""
+    if forward_ad._current_level >= 0 and any(
+            isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise ArgumentError("no forward-mode derivative: an argument carries a tangent")
     return torch.is_grad_enabled() and any(t is not None and getattr(t, "requires_grad", False)
                                            for t in ts)
 
