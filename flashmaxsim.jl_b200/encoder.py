@@ -249,9 +249,9 @@ def int8_linear(x, w: Int8Index, bias=None, out_dtype=None):
     else:
         if x.dtype not in _FLOAT:
             raise ArgumentError(f"int8_linear: unsupported dtype {x.dtype}")
-        if needs_grad(x, bias):
-            raise ArgumentError("int8_linear is forward-only (no autograd pullback)")
         xt, out_dtype = _lib.DTYPE_CODE[x.dtype], out_dtype or x.dtype
+    if needs_grad(x, xs, scales, bias):
+        raise ArgumentError("int8_linear is forward-only (no autograd pullback)")
     if out_dtype not in _FLOAT:
         raise ArgumentError(f"int8_linear: unsupported output dtype {out_dtype}")
     out, dim = codes.shape
