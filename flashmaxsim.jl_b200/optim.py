@@ -75,7 +75,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
     if dev.type != "cuda":
         raise ArgumentError("adamw_step runs on CUDA tensors only")
     eight = isinstance(exp_avgs[0], (tuple, list))
-    states = exp_avgs + exp_avg_sqs
+    states, scales = exp_avgs + exp_avg_sqs, []
     if eight:
         if not all(isinstance(s, (tuple, list)) and len(s) == 2 for s in states):
             raise ArgumentError("adamw_step: moments must all be tensors or all (codes, scales)")
@@ -113,7 +113,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
         if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
             raise ArgumentError("adamw_step: grad_scale must be a float32 tensor of one value")
         _checked(dev, [grad_scale])
-    torch.autograd.graph.increment_version(params + states + (copies or []))
+    torch.autograd.graph.increment_version(params + states + scales + (copies or []))
     args = (8 if eight else 32, n, table, int(step), float(lr), float(b1), float(b2),
             float(eps), float(weight_decay), int(seed) & 0xFFFFFFFF,
             None if grad_scale is None else grad_scale.data_ptr())
