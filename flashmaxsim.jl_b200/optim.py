@@ -45,7 +45,6 @@ def _dtypes(ts):
     return [t.dtype for t in ts]
 
 
-@torch.no_grad()
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.9, 0.999),
                eps=1e-8, weight_decay=1e-2, seed=0, copies=None, grad_scale=None):
     """One AdamW step (decoupled weight decay) in place over lists of tensors:
@@ -59,6 +58,11 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
     (16-bit tensors, or None) receive the new parameters in their type.  step
     counts from 1.  grad_scale, a float32 tensor of one value, multiplies the
     gradients (a clipping factor, an inverse loss scale)."""
+    _take(_plan(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, seed, copies, grad_scale))
+
+
+def _plan(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, seed, copies, grad_scale):
+    """Checks one step's arguments: its device, the tensors that it writes, the call's arguments."""
     params, grads = list(params), list(grads)
     exp_avgs, exp_avg_sqs = list(exp_avgs), list(exp_avg_sqs)
     n = len(params)
@@ -70,7 +74,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
     if not (0 <= b1 < 1 and 0 <= b2 < 1) or not eps >= 0 or int(step) < 1:
         raise ArgumentError("adamw_step: betas must be in [0, 1), eps >= 0 and step >= 1")
     if n == 0:
-        return
+        return None
     dev = params[0].device
     if dev.type != "cuda":
         raise ArgumentError("adamw_step runs on CUDA tensors only")
@@ -113,11 +117,17 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
         if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
             raise ArgumentError("adamw_step: grad_scale must be a float32 tensor of one value")
         _checked(dev, [grad_scale])
-    torch.autograd.graph.increment_version(params + states + scales + (copies or []))
-    args = (8 if eight else 32, n, table, int(step), float(lr), float(b1), float(b2),
-            float(eps), float(weight_decay), int(seed) & 0xFFFFFFFF,
-            None if grad_scale is None else grad_scale.data_ptr())
-    _run("fms_adamw_step", dev, *args)
+    written = params + states + scales + (copies or [])
+    return dev, written, (8 if eight else 32, n, table, int(step), float(lr), float(b1), float(b2),
+                          float(eps), float(weight_decay), int(seed) & 0xFFFFFFFF,
+                          None if grad_scale is None else grad_scale.data_ptr())
+
+
+def _take(plan):
+    if plan is not None:
+        dev, written, args = plan
+        torch.autograd.graph.increment_version(written)
+        _run("fms_adamw_step", dev, *args)
 
 
 def moments8(p):
@@ -156,19 +166,22 @@ class AdamW:
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             raise DimensionMismatch("AdamW: one gradient per parameter")
-        at = [k for k, g in enumerate(grads) if g is not None]
-        for k in at:
-            if self.exp_avgs[k] is None:
-                self.exp_avgs[k] = self._moment(self.params[k])
-                self.exp_avg_sqs[k] = self._moment(self.params[k])
-            self.steps[k] += 1
-        for t in sorted({self.steps[k] for k in at}):
-            pick = lambda ts: [ts[k] for k in at if self.steps[k] == t]  # noqa: B023, E731
-            adamw_step([p.detach() for p in pick(self.params)], pick(grads), pick(self.exp_avgs),
-                       pick(self.exp_avg_sqs), step=t, lr=self.lr, betas=self.betas, eps=self.eps,
-                       weight_decay=self.weight_decay, seed=self.seed,
-                       copies=None if self.copies is None else pick(self.copies),
-                       grad_scale=grad_scale)
+        groups = {}  # by the step that they are at
+        for k, g in enumerate(grads):
+            if g is not None:
+                groups.setdefault(self.steps[k] + 1, []).append(k)
+        plans = []  # all of them are checked before any is taken: a refused step changes nothing
+        for t, ks in sorted(groups.items()):
+            pick = lambda ts: [ts[k] for k in ks]  # noqa: B023, E731
+            m, v = ([s[k] if s[k] is not None else self._moment(self.params[k]) for k in ks]
+                    for s in (self.exp_avgs, self.exp_avg_sqs))
+            plans.append((t, ks, m, v, _plan(
+                pick(self.params), pick(grads), m, v, t, self.lr, self.betas, self.eps,
+                self.weight_decay, self.seed, None if self.copies is None else pick(self.copies), grad_scale)))
+        for t, ks, m, v, plan in plans:
+            _take(plan)
+            for k, a, b in zip(ks, m, v):
+                self.exp_avgs[k], self.exp_avg_sqs[k], self.steps[k] = a, b, t
 
     def zero_grad(self):
         for p in self.params:
