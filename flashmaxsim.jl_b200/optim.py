@@ -136,6 +136,17 @@ def moments8(p):
             torch.zeros(-(-p.numel() // BLOCK), dtype=torch.float32, device=p.device))
 
 
+def _parts(moment):
+    return list(moment) if isinstance(moment, (tuple, list)) else [moment]
+
+
+def _copy(moment, device=None):
+    if moment is None:
+        return None
+    c = [t.detach().to(t.device if device is None else device, copy=True).contiguous() for t in _parts(moment)]
+    return tuple(c) if isinstance(moment, (tuple, list)) else c[0]
+
+
 class AdamW:
     """AdamW over a list of parameters, its moments kept in `bits` (32 or 8) each.
 
@@ -188,11 +199,27 @@ class AdamW:
             p.grad = None
 
     def state_dict(self):
-        return {"steps": list(self.steps), "bits": self.bits, "exp_avgs": list(self.exp_avgs),
-                "exp_avg_sqs": list(self.exp_avg_sqs)}
+        """A copy of the state: later steps do not change it."""
+        return {"steps": list(self.steps), "bits": self.bits, "exp_avgs": list(map(_copy, self.exp_avgs)),
+                "exp_avg_sqs": list(map(_copy, self.exp_avg_sqs))}
 
     def load_state_dict(self, state):
-        if state["bits"] != self.bits or len(state["exp_avgs"]) != len(self.params):
+        """Takes up a copy of a state of this width and these parameters' sizes, from any
+        device; one that does not fit is refused and changes nothing."""
+        n = len(self.params)
+        steps, moments = list(state["steps"]), [list(state["exp_avgs"]), list(state["exp_avg_sqs"])]
+        if state["bits"] != self.bits or any(len(s) != n for s in (steps, *moments)):
             raise ArgumentError("AdamW: the state is of another width or number of parameters")
-        self.steps = list(state["steps"])
-        self.exp_avgs, self.exp_avg_sqs = list(state["exp_avgs"]), list(state["exp_avg_sqs"])
+        want = [torch.float8_e4m3fn, torch.float32] if self.bits == 8 else [torch.float32]
+        for p, t, m, v in zip(self.params, steps, *moments):
+            if t < 0 or (m is None) != (v is None) or (m is None) != (t == 0):
+                raise ArgumentError("AdamW: the state's counts and moments do not belong together")
+            sizes = [p.numel(), -(-p.numel() // BLOCK)][:len(want)]
+            for s in (m, v) if m is not None else ():
+                parts = _parts(s)
+                if len(parts) != len(want) or _dtypes(parts) != want:
+                    raise ArgumentError(f"AdamW: moments of {self.bits} bits must hold {want}")
+                if list(map(_numel, parts)) != sizes:
+                    raise DimensionMismatch("AdamW: a moment is not of its parameter's size")
+        self.exp_avgs, self.exp_avg_sqs = ([_copy(s, p.device) for s, p in zip(m, self.params)] for m in moments)
+        self.steps = steps

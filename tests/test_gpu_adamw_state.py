@@ -48,6 +48,71 @@ def test_a_refused_step_changes_nothing(fms, bits):
     assert same(opt.params, ref.params) and same(opt.exp_avgs, ref.exp_avgs) and same(opt.exp_avg_sqs, ref.exp_avg_sqs)
 
 
+@BITS
+def test_a_saved_state_is_taken_up_twice(fms, bits):
+    """Two optimisers from one dict step independently, and the dict keeps what it held."""
+    opt, g = make(fms, bits)
+    opt.step(g)
+    saved = opt.state_dict()
+    kept = [[tuple(u.clone() for u in s) if bits == 8 else s.clone() for s in saved[k]] for k in ("exp_avgs", "exp_avg_sqs")]
+    start = [t.clone() for t in opt.params]
+
+    def taken_up():
+        o = fms.AdamW([t.clone() for t in start], bits=bits, seed=1, **H)
+        o.load_state_dict(saved)
+        return o
+
+    a, b = taken_up(), taken_up()
+    for o in (opt, a, b):
+        for _ in range(2):
+            o.step(g)
+    assert opt.steps == a.steps == b.steps == [3, 3]
+    assert same(opt.params, a.params) and same(opt.params, b.params)
+    assert same(opt.exp_avgs, a.exp_avgs) and same(opt.exp_avgs, b.exp_avgs)
+    assert same(saved["exp_avgs"], kept[0]) and same(saved["exp_avg_sqs"], kept[1]) and saved["steps"] == [1, 1]
+    # back to the saved step
+    for t, s in zip(opt.params, start):
+        t.copy_(s)
+    opt.load_state_dict(saved)
+    for _ in range(2):
+        opt.step(g)
+    assert same(opt.params, a.params) and same(opt.exp_avgs, a.exp_avgs) and same(opt.exp_avg_sqs, a.exp_avg_sqs)
+
+
+@BITS
+def test_a_state_read_on_the_host(fms, bits):
+    """Moments that were loaded to the host go to their parameter's device."""
+    opt, g = make(fms, bits)
+    opt.step(g)
+    host = {k: [tuple(u.cpu() for u in s) if bits == 8 else s.cpu() for s in v] if k.startswith("exp") else v
+            for k, v in opt.state_dict().items()}
+    other = fms.AdamW([t.clone() for t in opt.params], bits=bits, seed=1, **H)
+    other.load_state_dict(host)
+    opt.step(g), other.step(g)
+    assert same(opt.params, other.params)
+
+
+@BITS
+def test_a_state_that_does_not_fit_is_refused(fms, bits):
+    opt, g = make(fms, bits)
+    opt.step(g)
+    good = opt.state_dict()
+    short = lambda s: tuple(u[:-1] for u in s) if bits == 8 else s[:-1]  # noqa: E731
+    other = lambda s: (s[0].float(), s[1]) if bits == 8 else s.half()  # noqa: E731
+    m = good["exp_avgs"]
+    before = [opt.steps, opt.exp_avgs, opt.exp_avg_sqs]
+    for err, bad in [(fms.ArgumentError, dict(good, steps=[1])),
+                     (fms.ArgumentError, dict(good, steps=[1, -1])),
+                     (fms.ArgumentError, dict(good, exp_avgs=m[:1])),
+                     (fms.ArgumentError, dict(good, exp_avg_sqs=good["exp_avg_sqs"][:1])),
+                     (fms.ArgumentError, dict(good, exp_avgs=[m[0], None])),
+                     (fms.ArgumentError, dict(good, exp_avgs=[m[0], other(m[1])])),
+                     (fms.DimensionMismatch, dict(good, exp_avgs=[short(m[0]), m[1]]))]:
+        with pytest.raises(err):
+            opt.load_state_dict(bad)
+        assert all(x is y for x, y in zip(before, [opt.steps, opt.exp_avgs, opt.exp_avg_sqs]))
+
+
 def test_versions_of_all_that_is_written(fms):
     p, g = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
     c = p.bfloat16()
