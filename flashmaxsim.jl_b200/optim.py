@@ -117,6 +117,15 @@ def _plan(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_dec
         if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
             raise ArgumentError("adamw_step: grad_scale must be a float32 tensor of one value")
         _checked(dev, [grad_scale])
+    # Two entries that write the same memory would race in the kernel.  (Empty tensors have
+    # no address, and a copy may be its parameter.)
+    lists = [p, m, v, c] + ([ms, vs] if eight else [])
+    starts = sum(lists, [])
+    if len(set(starts)) < len(starts):
+        lists[3] = [0 if a == b else a for a, b in zip(c, p)]
+        starts = [a for ts in lists for a, s in zip(ts, sizes) if s and a]
+        if len(set(starts)) < len(starts):
+            raise ArgumentError("adamw_step: a tensor that is written is named twice")
     written = params + states + scales + (copies or [])
     return dev, written, (8 if eight else 32, n, table, int(step), float(lr), float(b1), float(b2),
                           float(eps), float(weight_decay), int(seed) & 0xFFFFFFFF,

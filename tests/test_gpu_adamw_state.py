@@ -122,3 +122,32 @@ def test_versions_of_all_that_is_written(fms):
     fms.adamw_step([p], [g], [m], [v], step=1, copies=[c])
     assert all(t._version > b for t, b in zip(written, before))
     assert g._version == 0
+
+
+def test_a_tensor_named_twice_is_refused(fms):
+    """Two entries of one launch that write the same memory would race."""
+    z = lambda n=512: torch.zeros(n, device="cuda")  # noqa: E731
+    p, q, g = z(), z(), torch.ones(512, device="cuda")
+    m, v = [z(), z()], [z(), z()]
+    e = fms.moments8(p)
+    for f in (lambda: fms.adamw_step([p, p], [g, g], m, v, step=1),
+              lambda: fms.adamw_step([p, q], [g, g], [m[0], m[0]], v, step=1),
+              lambda: fms.adamw_step([p, q], [g, g], m, [v[0], m[1]], step=1),
+              lambda: fms.adamw_step([p], [g], [(e[0], e[1])], [(fms.moments8(p)[0], e[1])], step=1),
+              lambda: fms.adamw_step([p.bfloat16()] * 2, [g, g], m, v, step=1),
+              lambda: fms.AdamW([p, p]).step([g, g])):
+        with pytest.raises(fms.ArgumentError, match="twice"):
+            f()
+    assert not p.any() and not m[0].any()
+    # shared gradients are only read; empty tensors may have any address
+    fms.adamw_step([p, q, z(0), z(0)], [g, g, z(0), z(0)], m + [z(0), z(0)], v + [z(0), z(0)], step=1)
+    assert torch.equal(p, q) and p.any()
+
+
+def test_a_copy_may_be_its_parameter(fms):
+    p, g = torch.ones(300, device="cuda").bfloat16(), torch.ones(300, device="cuda")
+    q = p.clone()
+    m, v, m2, v2 = (torch.zeros(300, device="cuda") for _ in range(4))
+    fms.adamw_step([p], [g], [m], [v], step=1, copies=[p])
+    fms.adamw_step([q], [g], [m2], [v2], step=1)
+    assert torch.equal(p, q)
