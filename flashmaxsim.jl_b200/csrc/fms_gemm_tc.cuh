@@ -461,7 +461,7 @@ __device__ __forceinline__ void load_row32(const T* p, uint32_t (&v)[16], int n)
   if (n >= 32) {
 #pragma unroll
     for (int q = 0; q < 2; ++q)
-      asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+      asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                    : "=r"(v[8 * q]), "=r"(v[8 * q + 1]), "=r"(v[8 * q + 2]), "=r"(v[8 * q + 3]), "=r"(v[8 * q + 4]),
                      "=r"(v[8 * q + 5]), "=r"(v[8 * q + 6]), "=r"(v[8 * q + 7])
                    : "l"(p + 16 * q));

@@ -347,12 +347,12 @@ __global__ void __launch_bounds__(128) few_kernel(const T* x, const T* wg, const
     const uint4* b = reinterpret_cast<const uint4*>(wu + (int64_t)f * dim);
 #pragma unroll 3
     for (int k = lane; k < dim / 8; k += 32) {
-      const uint4 wa = __ldg(a + k), wb = __ldg(b + k);
+      const uint4 wa = a[k], wb = b[k];
       const uint32_t ga[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
         if (r >= rows) break;
-        const uint4 xv = __ldg(reinterpret_cast<const uint4*>(x + (int64_t)r * dim) + k);
+        const uint4 xv = reinterpret_cast<const uint4*>(x + (int64_t)r * dim)[k];
         const uint32_t xs[4] = {xv.x, xv.y, xv.z, xv.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

@@ -3,6 +3,10 @@
 // dependency_wait() before it reads or writes global memory: it returns when everything
 // the earlier kernel wrote is there.  Right after it the kernel lets the next one begin in
 // the same way, which then takes the SMs as they fall free; about 2 us a launch.
+//
+// Such a kernel reads global memory by ordinary loads only: a load through the read-only
+// path (__ldg, ld.global.nc) is for memory that nobody writes while the kernel runs, and
+// this one runs already while the earlier one writes.
 #pragma once
 #include <cuda_runtime.h>
 

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* x, int64_t rows,
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     v[i] = make_uint4(0, 0, 0, 0);
-    if (real && (i * TPR + tid) * N < K) v[i] = __ldg(xt + i * TPR + tid);
+    if (real && (i * TPR + tid) * N < K) v[i] = xt[i * TPR + tid];
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(256) few_kernel(const X* x, const float* x_sca
 #pragma unroll 2
     for (int k = lane * VEC; k < K; k += 32 * VEC) {
       if constexpr (VEC == 16) {
-        const int4 v = __ldg(reinterpret_cast<const int4*>(w + k));
+        const int4 v = *reinterpret_cast<const int4*>(w + k);
 #pragma unroll
         for (int t = 0; t < NTOK; ++t) {
           if (t >= rows) break;
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(256) few_kernel(const X* x, const float* x_sca
           acc[t] = __dp4a(v.x, q.x, __dp4a(v.y, q.y, __dp4a(v.z, q.z, __dp4a(v.w, q.w, acc[t]))));
         }
       } else if constexpr (VEC == 4) {
-        const int v = __ldg(reinterpret_cast<const int*>(w + k));
+        const int v = *reinterpret_cast<const int*>(w + k);
 #pragma unroll
         for (int t = 0; t < NTOK; ++t) {
           if (t >= rows) break;
@@ -262,7 +262,7 @@ struct ScaleEpi {
   static __device__ __forceinline__ void run(const Params& p, const gemm::Tile& t, int64_t row, int half, uint32_t addr,
                                              const Ahead<BN>&, unsigned char* stage, Release release) {
     const int lane = threadIdx.x & 31;
-    const float sx = row < p.rows ? __ldg(p.sx + row) : 0.f;
+    const float sx = row < p.rows ? p.sx[row] : 0.f;
 #pragma unroll 1
     for (int c = half * (BN / 64); c < (half + 1) * (BN / 64); ++c) {
       __syncwarp();
@@ -277,7 +277,7 @@ struct ScaleEpi {
       if (p.wide && col + 32 <= p.cols) {
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
-          const float4 w = __ldg(reinterpret_cast<const float4*>(p.sw + col + i));
+          const float4 w = *reinterpret_cast<const float4*>(p.sw + col + i);
           f[i] = (sx * w.x) * (float)(int32_t)v[i];
           f[i + 1] = (sx * w.y) * (float)(int32_t)v[i + 1];
           f[i + 2] = (sx * w.z) * (float)(int32_t)v[i + 2];
@@ -288,7 +288,7 @@ struct ScaleEpi {
 #pragma unroll
           for (int i = 0; i < 32; i += N) {
             float b[N];
-            Vec<Y>::get(__ldg(reinterpret_cast<const uint4*>(p.bias + col + i)), b);
+            Vec<Y>::get(*reinterpret_cast<const uint4*>(p.bias + col + i), b);
 #pragma unroll
             for (int j = 0; j < N; ++j) f[i + j] += b[j];
           }
@@ -297,7 +297,7 @@ struct ScaleEpi {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           const int at = min(col + i, p.cols - 1);
-          f[i] = (sx * __ldg(p.sw + at)) * (float)(int32_t)v[i];
+          f[i] = (sx * p.sw[at]) * (float)(int32_t)v[i];
           if (p.bias) f[i] += Tr<Y>::to(p.bias[at]);
         }
       }

@@ -136,7 +136,7 @@ __device__ __forceinline__ void load_vec(const void* p, int vdt, int64_t at, int
 #pragma unroll
     for (int e = 0; e < 2 * N; ++e) {
       const int c = (e / VEC * tpr + tid) * VEC + e % VEC;
-      const float v = c >= D ? 0.f : WIDE || vdt == FMS_F32 ? __ldg(q + c) : Tr<T>::to(u[c]);
+      const float v = c >= D ? 0.f : WIDE || vdt == FMS_F32 ? q[c] : Tr<T>::to(u[c]);
       if (e & 1) f[e >> 1].y = v;
       else f[e >> 1].x = v;
     }
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(512, 1) backward_kernel(Params p) {
     if (p.dy) ry.load(static_cast<const T*>(p.dy) + r * D, tid, tpr, D);
     if (p.dz) rd.load(static_cast<const T*>(p.dz) + r * D, tid, tpr, D);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) st[k] = __ldg(p.stats + k * p.rows + r);
+    for (int k = 0; k < 4; ++k) st[k] = p.stats[k * p.rows + r];
   };
   fetch(r0);
   for (int64_t r = r0; r < r1; ++r) {
