@@ -350,7 +350,7 @@ int fms_int8_linear_fwd(int x_dtype, const void* x, const float* x_scales, const
    16-bit type as well.  bits 32: m and v are float32.  bits 8: m and v hold e4m3
    codes of m and of sqrt(v), m_scales and v_scales one float32 per 256 values
    (value = code * scale); with eps 0 a value whose second moment is zero becomes
-   NaN.  Codes are rounded stochastically from (seed, step, the
+   NaN.  What the step writes must not overlap: the tensors are stepped at once.  Codes are rounded stochastically from (seed, step, the
    tensor's place in the list, the value's place in the tensor).  `tensors` is a
    host array that the call reads before it returns. */
 typedef struct fms_adamw_tensor {
